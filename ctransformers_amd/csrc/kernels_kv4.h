@@ -46,8 +46,8 @@ struct Kv4Attn {
     Kv4Rows q;
     void* out;
     long long o_row, o_head;
-    float* ws;               // partial results: [row tile][split][rows of a tile][head_dim + 2]
-    int out_type, n_head, rep, tiles, nsplit, min_blocks;   // rep: query heads of a KV head; tiles: row tiles of a (sequence, KV head)
+    float* ws;               // partial results, head_dim + 2 floats a row: [share][2][rows of a tile] or [row tile][split][rows of a tile]
+    int out_type, n_head, rep, tiles, nsplit, min_blocks, want_parts;   // rep: query heads of a KV head; tiles: row tiles of a (sequence, KV head)
     float scale;
 };
 
@@ -82,6 +82,19 @@ DEV uint32_t bits_of(float f) { return __builtin_bit_cast(uint32_t, f); }
 DEV float float_of(uint32_t u) { return __builtin_bit_cast(float, u); }
 DEV void atomic_add_i32(int* p, int v) { (void)atomicAdd(p, v); }
 #endif
+// an index that the compiler has to take as new: what follows from it is computed where it is used and not kept in registers around an outer loop
+#ifdef CT_EMU
+static inline int kv4_anew(int v) { return v; }
+#else
+DEV int kv4_anew(int v) { asm volatile("" : "+v"(v)); return v; }
+#endif
+// An entry of table, lens or cu: constant while a kernel runs, so that a load with a uniform index goes through the scalar cache — as a vector load it would wait
+// behind every K and V load in flight.
+#ifdef CT_EMU
+static inline int kv4_entry(const int* p, long long i) { return p[i]; }
+#else
+DEV int kv4_entry(const int* p, long long i) { return ((const __attribute__((address_space(4))) int*)p)[i]; }
+#endif
 DEV float kv4_load_any(const void* p, long long i, int type) {
     if (type == KV4_F32) return ((const float*)p)[i];
     const uint16_t b = ((const uint16_t*)p)[i];
@@ -96,10 +109,17 @@ DEV void kv4_store_any(void* p, long long i, int type, float f) {
     if (type == KV4_F32) ((float*)p)[i] = f;
     else ((uint16_t*)p)[i] = type == KV4_F16 ? f32_to_f16_bits(f) : bf16_of(f);
 }
-// eight neighbouring dims
+// eight neighbouring dims of a 16-bit type as they are
+DEV u32x4 kv4_load8_raw(const Kv4Rows& r, long long at) {
+    if (r.vec) return ld16((const uint16_t*)r.p + at);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = (uint32_t)((const uint16_t*)r.p)[at + 2 * j * r.dim] | ((uint32_t)((const uint16_t*)r.p)[at + (2 * j + 1) * r.dim] << 16);
+    return u32x4_of(w[0], w[1], w[2], w[3]);
+}
 DEV void kv4_load8(float (&x)[8], const Kv4Rows& r, long long at) {
-    if (r.vec && r.type != KV4_F32) {
-        const u32x4 w = ld16((const uint16_t*)r.p + at);
+    if (r.type != KV4_F32) {
+        const u32x4 w = kv4_load8_raw(r, at);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (r.type == KV4_F16) { x[2 * j] = f16_bits_to_f32((uint16_t)(w[j] & 0xFFFFu)); x[2 * j + 1] = f16_bits_to_f32((uint16_t)(w[j] >> 16)); }
@@ -114,7 +134,52 @@ DEV void kv4_load8(float (&x)[8], const Kv4Rows& r, long long at) {
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = kv4_load_any(r.p, at + j * r.dim, r.type);
+        for (int j = 0; j < 8; ++j) x[j] = ((const float*)r.p)[at + j * r.dim];
+    }
+}
+// A query row's pieces as halves: N pieces of eight dims, piece k at at + 8 * (k * step + lane's), dims from head_dim on are zeros.  Rows that f16 may not hold (bf16,
+// f32) are scaled by a power of two that brings the row's largest value into [1, 2) — all lanes that hold pieces of a row agree on it through `across` — so that bf16
+// stays exact but for values below 2^-17 of the largest.  Returns the inverse of the scale.
+template <int N, class Across> DEV float kv4_query(u32x4 (&q)[N], const Kv4Rows& r, long long at, int d0, int step, int head_dim, bool on, Across across) {
+    if (r.type == KV4_F16) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const bool in = on && d0 + step * k < head_dim;
+            q[k] = kv4_load8_raw(r, in ? at + d0 + step * k : at);
+            if (!in) q[k] = u32x4_of(0, 0, 0, 0);
+        }
+        return 1.0f;
+    }
+    float x[N][8], big = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const bool in = on && d0 + step * k < head_dim;
+        kv4_load8(x[k], r, in ? at + d0 + step * k : at);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { x[k][j] = in ? x[k][j] : 0.0f; big = fmaxf(big, fabsf(x[k][j])); }
+    }
+    big = across(big);
+    float up = 1.0f, down = 1.0f;
+    const int e = (int)((bits_of(big) >> 23) & 255u);
+    if (e > 0 && e < 254) { up = float_of((uint32_t)(254 - e) << 23); down = float_of((uint32_t)e << 23); }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        q[k] = u32x4_of(kv4_cvt2(x[k][0] * up, x[k][1] * up), kv4_cvt2(x[k][2] * up, x[k][3] * up), kv4_cvt2(x[k][4] * up, x[k][5] * up), kv4_cvt2(x[k][6] * up, x[k][7] * up));
+    return down;
+}
+// eight neighbouring dims out; vec: as for loads
+DEV void kv4_store8(void* p, long long at, int type, int vec, const float (&x)[8]) {
+    if (vec && type != KV4_F32) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[j] = type == KV4_F16 ? kv4_cvt2(x[2 * j], x[2 * j + 1]) : (uint32_t)bf16_of(x[2 * j]) | ((uint32_t)bf16_of(x[2 * j + 1]) << 16);
+        *(u32x4*)((uint16_t*)p + at) = u32x4_of(w[0], w[1], w[2], w[3]);
+    } else if (vec) {
+        *(u32x4*)((float*)p + at) = u32x4_of(bits_of(x[0]), bits_of(x[1]), bits_of(x[2]), bits_of(x[3]));
+        *(u32x4*)((float*)p + at + 4) = u32x4_of(bits_of(x[4]), bits_of(x[5]), bits_of(x[6]), bits_of(x[7]));
+    } else {
+        for (int j = 0; j < 8; ++j) kv4_store_any(p, at + j, type, x[j]);
     }
 }
 template <int N> DEV void kv4_ldw(uint32_t (&d)[N], const uint8_t* p) {
@@ -131,28 +196,36 @@ template <int N> DEV void kv4_ldw(uint32_t (&d)[N], const uint8_t* p) {
 }
 // the packed rows [lo, hi) of sequence b and its length; rows outside the packed tensor are not there
 DEV void kv4_seq(const Kv4Cache& c, int b, int& lo, int& hi, int& len) {
-    lo = c.cu ? c.cu[b] : 0;
-    hi = c.cu ? c.cu[b + 1] : c.total;
+    lo = c.cu ? kv4_entry(c.cu, b) : 0;
+    hi = c.cu ? kv4_entry(c.cu, b + 1) : c.total;
     if (lo < 0) lo = 0;
     if (hi > c.total) hi = c.total;
     if (hi < lo) hi = lo;
-    const long long n = (long long)c.lens[b] + c.len_add;
+    const long long n = (long long)kv4_entry(c.lens, b) + c.len_add;
     len = n < 0 ? 0 : n > (1 << 30) ? 1 << 30 : (int)n;
 }
 // block `blk` of head h of sequence b, null where the table names no page
 DEV uint8_t* kv4_block(const Kv4Cache& c, int b, int h, int blk) {
     const int pi = blk >> c.bshift;
     if (blk < 0 || pi >= c.table_width) return nullptr;
-    const int pid = c.table[(long long)b * c.table_stride + pi];
+    const int pid = kv4_entry(c.table, (long long)b * c.table_stride + pi);
     if ((unsigned)pid >= (unsigned)c.n_pages) return nullptr;
     const long long in_page = ((long long)h << c.bshift) + (blk & ((1 << c.bshift) - 1));
     return c.pages + (long long)pid * c.page_stride + in_page * c.groups * kKv4Block;
 }
 
+// the same in two steps, for loops that look a table entry up well before they need the block: the entry, and the block's address in that page
+DEV int kv4_page_of(const Kv4Cache& c, int b, int blk) { return kv4_entry(c.table, (long long)b * c.table_stride + (blk >> c.bshift)); }   // blk < table_width << bshift
+DEV const uint8_t* kv4_in_page(const Kv4Cache& c, int pid, int h, int blk) {
+    if ((unsigned)pid >= (unsigned)c.n_pages) return nullptr;
+    return c.pages + (long long)pid * c.page_stride + (((long long)h << c.bshift) + (blk & ((1 << c.bshift) - 1))) * c.groups * kKv4Block;
+}
+
 // ---- rows into the cache --------------------------------------------------------------------------------------------------------------------------
 // One workgroup per (block, head) that new rows fall into: it alone writes that block, so a V dword that keeps older tokens is read, changed and written without
-// atomics.  A thread quantizes one group of one token; K codes and scales go straight out, V codes cross the workgroup through LDS (eight tokens to a dword).
-// Memory-bound for prompts: the rows are read once, 16 bytes a lane, and 4.5 bits a value written.
+// atomics.  A lane takes eight dims (16 bytes of a half row, so that a wave reads whole lines), four lanes a group; they agree on the largest value by two quad
+// exchanges.  K codes and scales go straight out, V codes cross the workgroup through LDS (eight tokens to a dword).  All loads of a lane are issued before the
+// first value is used.
 template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
     __shared__ uint32_t vcode[32][8 * G + 1];   // V codes as bytes [token][dim]; + 1: tokens in different banks
     __shared__ uint16_t sc[2][32][G];
@@ -167,52 +240,62 @@ template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const 
     uint8_t* dst = kv4_block(c, b, h, blk);
     if (!dst) return;
     const int t_lo = start > blk * 32 ? start - blk * 32 : 0, t_hi = len - blk * 32 < 32 ? len - blk * 32 : 32;   // the new tokens of this block
-    for (int t = tid; t < 32; t += 256) poison[t] = 0;
+    if (tid < 32) poison[tid] = 0;
+    // piece `it` of 256 G: half (K, V), token, group, eight dims
+    float x[G][8];
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+        const int it = tid + 256 * k, half = it / (128 * G), t = (it / (4 * G)) & 31, d0 = 8 * (it % (4 * G));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[k][j] = 0.0f;
+        if (t < t_lo || t >= t_hi || d0 >= c.head_dim) continue;
+        const long long at = (long long)(lo + blk * 32 + t - start);
+        if (half) kv4_load8(x[k], a.v, at * a.v.row + (long long)h * a.v.head + d0 * a.v.dim);
+        else kv4_load8(x[k], a.k, at * a.k.row + (long long)h * a.k.head + d0 * a.k.dim);
+    }
     __syncthreads();
-    for (int it = tid; it < 2 * 32 * G; it += 256) {
-        const int half = it / (32 * G), t = (it / G) & 31, g = it % G;
-        if (t < t_lo || t >= t_hi) continue;
-        const Kv4Rows& r = half ? a.v : a.k;
-        const long long at = (long long)(lo + blk * 32 + t - start) * r.row + (long long)h * r.head;
-        float x[32], top = 0.0f, big = 0.0f;
-        bool nan = false;
 #pragma unroll
-        for (int o = 0; o < 4; ++o) {
-            const int d0 = 32 * g + 8 * o;
-            float y[8];
-            if (d0 < c.head_dim) kv4_load8(y, r, at + d0 * r.dim);
-            else for (int j = 0; j < 8; ++j) y[j] = 0.0f;
+    for (int k = 0; k < G; ++k) {
+        const int it = tid + 256 * k, half = it / (128 * G), t = (it / (4 * G)) & 31, g = (it / 4) % G, o = it & 3;
+        const bool on = t >= t_lo && t < t_hi;
+        float top = 0.0f;
+        int nan = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v = y[j] > 65504.0f ? 65504.0f : y[j] < -65504.0f ? -65504.0f : y[j];
-                nan = nan || v != v;
-                x[8 * o + j] = v;
-                if (fabsf(v) > big) { big = fabsf(v); top = v; }
-            }
+        for (int j = 0; j < 8; ++j) {
+            const float v = x[k][j] > 65504.0f ? 65504.0f : x[k][j] < -65504.0f ? -65504.0f : x[k][j];
+            nan |= v != v;
+            x[k][j] = v;
+            if (fabsf(v) > fabsf(top)) top = v;
         }
+        // the quad's largest, the first of equals (the four lanes hold the group's dims in order)
+        const float t1 = lane_xor1(top);
+        top = (o & 1) ? (fabsf(t1) >= fabsf(top) ? t1 : top) : (fabsf(t1) > fabsf(top) ? t1 : top);
+        const float t2 = lane_xor2(top);
+        top = (o & 2) ? (fabsf(t2) >= fabsf(top) ? t2 : top) : (fabsf(t2) > fabsf(top) ? t2 : top);
+        nan |= lane_xor1(nan);
+        nan |= lane_xor2(nan);
         const float d = top / -8.0f;
         const uint16_t dh = f32_to_f16_bits(d);
         const float inv = (dh & 0x7FFFu) ? 1.0f / d : 0.0f;     // a scale that f16 has as 0: every value is 0
-        uint32_t w[4] = {0, 0, 0, 0}, bytes[8];
+        uint32_t w = 0, lo4 = 0, hi4 = 0;
 #pragma unroll
-        for (int o = 0; o < 4; ++o) {
-            bytes[2 * o] = bytes[2 * o + 1] = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float f = x[8 * o + j] * inv + 8.5f;      // two roundings, as the reference's expression has
-                const int q = nan ? 8 : (int)f > 15 ? 15 : (int)f;
-                w[o] |= (uint32_t)q << (4 * (j / 2) + 16 * (j & 1));
-                bytes[2 * o + j / 4] |= (uint32_t)q << (8 * (j & 3));
-            }
+        for (int j = 0; j < 8; ++j) {
+            const float f = x[k][j] * inv + 8.5f;               // two roundings, as the reference's expression has
+            const int q = nan ? 8 : (int)f > 15 ? 15 : (int)f;
+            w |= (uint32_t)q << (4 * (j / 2) + 16 * (j & 1));
+            if (j < 4) lo4 |= (uint32_t)q << (8 * j);
+            else hi4 |= (uint32_t)q << (8 * (j - 4));
         }
-        if (nan) poison[t] = 1;
-        sc[half][t][g] = dh;
+        if (!on) continue;
+        if (o == 0) {
+            if (nan) poison[t] = 1;
+            sc[half][t][g] = dh;
+        }
         if (half) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) vcode[t][8 * g + j] = bytes[j];
+            vcode[t][8 * g + 2 * o] = lo4;
+            vcode[t][8 * g + 2 * o + 1] = hi4;
         } else {
-#pragma unroll
-            for (int o = 0; o < 4; ++o) ((uint32_t*)dst)[(4 * t + o) * G + g] = w[o];
+            ((uint32_t*)dst)[(4 * t + o) * G + g] = w;
         }
     }
     __syncthreads();
@@ -250,30 +333,47 @@ template <int G> __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv
     if (blk * 32 >= len || hi == lo) return;
     const uint8_t* src = kv4_block(c, b, h, blk);
     const int t_lo = start > blk * 32 ? start - blk * 32 : 0, t_hi = len - blk * 32 < 32 ? len - blk * 32 : 32;
-    for (int it = tid; it < 32 * 4 * G; it += 256) {   // K: eight dims of one token
-        const int t = it / (4 * G), i = (it / G) & 3, g = it % G, d0 = 32 * g + 8 * i;
+#pragma unroll
+    for (int k = 0; k < G; ++k) {   // pieces as in kv4_append_kernel
+        const int it = tid + 256 * k, half = it / (128 * G), t = (it / (4 * G)) & 31, g = (it / 4) % G, o = it & 3, d0 = 32 * g + 8 * o;
         if (t < t_lo || t >= t_hi || d0 >= c.head_dim) continue;
-        const long long at = (long long)(lo + blk * 32 + t - start) * a.k.row + (long long)h * a.k.head + d0;
-        const uint32_t w = src ? ((const uint32_t*)src)[it] : 0x88888888u;
-        const float d = src ? f16_bits_to_f32(((const uint16_t*)(src + 1024 * G))[(((t / 16) * 4 + (t & 15) / 4) * G + g) * 4 + (t & 3)]) : 0.0f;
-        for (int e = 0; e < 8; ++e) kv4_store_any((void*)a.k.p, at + e, a.k.type, d * (float)((int)((w >> (4 * (e / 2) + 16 * (e & 1))) & 15u) - 8));
-    }
-    for (int it = tid; it < 32 * 4 * G; it += 256) {   // V: the same eight dims, one nibble of each of their dwords
-        const int t = it / (4 * G), g = (it / 4) % G, d0 = 32 * g + 8 * (it & 3), i = (t & 15) / 4, e = (t & 3) + 4 * (t / 16);
-        if (t < t_lo || t >= t_hi || d0 >= c.head_dim) continue;
-        const long long at = (long long)(lo + blk * 32 + t - start) * a.v.row + (long long)h * a.v.head + d0;
-        const float d = src ? f16_bits_to_f32(((const uint16_t*)(src + 1088 * G))[(i * G + g) * 8 + e]) : 0.0f;
-        const uint32_t* vd = (const uint32_t*)(src ? src + 512 * G : nullptr) + (src ? i * 32 * G + d0 : 0);
-        for (int j = 0; j < 8; ++j)
-            kv4_store_any((void*)a.v.p, at + j, a.v.type, src ? d * (float)((int)((vd[j] >> (4 * (e / 2) + 16 * (e & 1))) & 15u) - 8) : 0.0f);
+        const int i = (t & 15) / 4, e = (t & 3) + 4 * (t / 16);
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (src && half) {          // one nibble of each of the eight dims' dwords
+            const float d = f16_bits_to_f32(((const uint16_t*)(src + 1088 * G))[(i * G + g) * 8 + e]);
+            const uint8_t* vd = src + 512 * G + (i * 32 * G + d0) * 4;
+            const u32x4 w0 = ld16(vd), w1 = ld16(vd + 16);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = d * (float)((int)(((j < 4 ? w0[j & 3] : w1[j & 3]) >> (4 * (e / 2) + 16 * (e & 1))) & 15u) - 8);
+        } else if (src) {
+            const float d = f16_bits_to_f32(((const uint16_t*)(src + 1024 * G))[(((t / 16) * 4 + i) * G + g) * 4 + (t & 3)]);
+            const uint32_t w = ((const uint32_t*)src)[(4 * t + o) * G + g];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = d * (float)((int)((w >> (4 * (j / 2) + 16 * (j & 1))) & 15u) - 8);
+        }
+        const long long at = (long long)(lo + blk * 32 + t - start);
+        if (half) kv4_store8((void*)a.v.p, at * a.v.row + (long long)h * a.v.head + d0, a.v.type, a.v.vec, x);
+        else kv4_store8((void*)a.k.p, at * a.k.row + (long long)h * a.k.head + d0, a.k.type, a.k.vec, x);
     }
 }
 
 // ---- attention ------------------------------------------------------------------------------------------------------------------------------------
 // The query rows of a (sequence, KV head) are r = token * rep + head, tiles of them share a workgroup; row r sees the positions below
-// len - rows + token + 1.  The blocks of a tile are divided over `nsplit` workgroups at most; how many of them have work follows from the sequence's own length.
+// len - rows + token + 1.  The blocks that a tile sees are divided into parts of `per` blocks, one workgroup each, `nsplit` of them at most (the grid); a part is
+// as long as it has to be for all of the call's parts to be about `want_parts`, whatever the sequences' lengths are: they are only known on the device.
 struct Kv4Range { int nq, n_rows, first_tok, len, lo, nb, per, parts; };
-DEV Kv4Range kv4_range(const Kv4Attn& a, int b, int tile, int tile_rows) {
+DEV int kv4_part(const Kv4Attn& a) {   // every lane of the wave calls it
+    if (a.nsplit <= 1) return 1;
+    long long sum = 0;
+    for (int b = lane_id(); b < a.c.n_seq; b += 64) {
+        const long long n = (long long)a.c.lens[b] + a.c.len_add;
+        sum += n < 0 ? 0 : (n + 31) / 32;
+    }
+    sum = wave_sum(sum) * a.c.n_head_kv * a.tiles;
+    const long long per = (sum + a.want_parts - 1) / a.want_parts;
+    return uniform_int((int)(per < a.min_blocks ? a.min_blocks : per > (1 << 25) ? 1 << 25 : per));
+}
+DEV Kv4Range kv4_range(const Kv4Attn& a, int b, int tile, int tile_rows, int part) {
     Kv4Range r;
     int lo, hi;
     kv4_seq(a.c, b, lo, hi, r.len);
@@ -287,9 +387,70 @@ DEV Kv4Range kv4_range(const Kv4Attn& a, int b, int tile, int tile_rows) {
     r.nb = seen > 0 ? (seen + 31) / 32 : 0;
     if (r.nb > a.c.table_width << a.c.bshift) r.nb = a.c.table_width << a.c.bshift;   // what the table has no room for is absent
     r.per = (r.nb + a.nsplit - 1) / a.nsplit;
-    if (r.per < a.min_blocks) r.per = a.min_blocks;
+    if (r.per < part) r.per = part;
     r.parts = (r.nb + r.per - 1) / r.per;
     return r;
+}
+
+// kv4_decode_kernel: the work of all units — a unit is a (sequence, KV head, row tile) — stands in one line, which is cut into equal shares, one per workgroup, as
+// many as are resident at once.  So every workgroup has the same work whatever the sequences' lengths are.  A unit's work is its blocks and, before them, kUnitCost
+// blocks' worth for beginning and ending it (~6 us: the queries, the first loads, the waves' results joined; four waves stream a block each in about that time).
+// Only the first and the last unit of a share can be a part of one; a part that does not begin its unit goes to the share's first place in the workspace, one that
+// begins it to the second, whole units go straight out.  The line follows from lens and cu, which only the device knows: every wave sums it up for itself.
+constexpr int kUnitCost = 4;
+struct Kv4Line { int before, all, per; };                     // (the host refuses tables with room for 2^31 blocks)
+DEV int kv4_unit_blocks(const Kv4Attn& a, int nq, int len) {   // blocks of each of a sequence's units (one, all masked, where there is nothing to see), 0: no rows
+    if (nq <= 0) return 0;
+    const int cap = a.c.table_width << a.c.bshift, nb = (len + 31) / 32;
+    return nb < 1 ? 1 : nb > cap ? (cap < 1 ? 1 : cap) : nb;
+}
+DEV int kv4_tiles(const Kv4Attn& a, int nq, int tile_rows) {
+    const int t = (nq * a.rep + tile_rows - 1) / tile_rows;    // (2^24 rows of 2^6 heads at most: the host's check)
+    return t < a.tiles ? t : a.tiles;                          // max_rows bounds the tiles
+}
+DEV int kv4_seq_work(const Kv4Attn& a, int tile_rows, int b) {
+    if (b >= a.c.n_seq) return 0;
+    int lo, hi, len;
+    kv4_seq(a.c, b, lo, hi, len);
+    const int nb = kv4_unit_blocks(a, hi - lo, len);
+    return nb ? (nb + kUnitCost) * kv4_tiles(a, hi - lo, tile_rows) * a.c.n_head_kv : 0;
+}
+// all the work of the line, and what lies before sequence `stop`
+DEV Kv4Line kv4_line(const Kv4Attn& a, int tile_rows, int stop) {
+    int all = 0, before = 0;
+    for (int b = lane_id(); b < ((a.c.n_seq + 63) & ~63); b += 64) {
+        const int n = kv4_seq_work(a, tile_rows, b);
+        all += n;
+        before += b < stop ? n : 0;
+    }
+    Kv4Line r;
+    r.all = uniform_int(wave_sum_fast(all));
+    r.before = stop > 0 ? uniform_int(wave_sum_fast(before)) : 0;
+    const int per = (int)(((long long)r.all + a.want_parts - 1) / a.want_parts);
+    r.per = per < a.min_blocks + kUnitCost ? a.min_blocks + kUnitCost : per;
+    return r;
+}
+// the sequence that place x of the line belongs to, and where that sequence begins
+DEV int kv4_find(const Kv4Attn& a, int tile_rows, int x, int& begin) {
+    int at = 0;
+    for (int b0 = 0; b0 < a.c.n_seq; b0 += 64) {
+        const int lane = lane_id(), n = kv4_seq_work(a, tile_rows, b0 + lane);
+        int sum = n;                                           // inclusive
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl(sum, lane >= d ? lane - d : lane);
+            if (lane >= d) sum += y;
+        }
+        const unsigned long long in = __ballot(n > 0 && x < at + sum);
+        if (in) {
+            const int l = __ffsll(in) - 1;
+            begin = uniform_int(at + __shfl(sum - n, l));
+            return b0 + l;
+        }
+        at += __shfl(sum, 63);
+    }
+    begin = uniform_int(at);
+    return a.c.n_seq;
 }
 
 // Eight halves of the dword's codes minus 8, times the scales of their tokens (or one scale for all): f16 products, one rounding (2^-11 of a value whose step is
@@ -306,26 +467,28 @@ DEV u32x4 kv4_values(uint32_t w, uint32_t s0, uint32_t s1, uint32_t s2, uint32_t
 // K's codes enter as f16 SUBNORMALS, the 16-bit integers themselves (code * 2^-24: no conversion); -8 * sum(Q) is the product's C operand and the group's scale
 // multiplies the 32-dim product in f32, so K is used exactly.  Maximum, sum and O stay per lane in f32; the maximum is raised (and O rescaled) only when a score
 // passes it by more than 2^8, so most blocks exchange nothing between lanes (p <= 256 fits f16 as well as p <= 1 does).
-// The block after the one being computed is in flight in registers (40 dwords a lane at 128 dims).
-template <int G> struct Kv4Raw { uint32_t kc[2][G], ks[2][2 * G], vc[2 * G], vs[2 * G + 2 * (G & 1)]; };
-template <int G> DEV void kv4_fetch(Kv4Raw<G>& r, const uint8_t* blk, int m, int i) {
+// The next block's K is fetched into the registers of this one's as soon as its scores are there, its V after the V product: 40 dwords a lane at 128 dims for a
+// block in flight, which leaves room for four waves a SIMD.
+template <int G> DEV void kv4_fetch_k(uint32_t (&kc)[2][G], uint32_t (&ks)[2][2 * G], const uint8_t* blk, int m, int i) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        kv4_ldw<G>(r.kc[t], blk + (((t * 16 + m) * 4 + i) * G) * 4);
-        kv4_ldw<2 * G>(r.ks[t], blk + 1024 * G + ((t * 4 + i) * G) * 8);
+        kv4_ldw<G>(kc[t], blk + (((t * 16 + m) * 4 + i) * G) * 4);
+        kv4_ldw<2 * G>(ks[t], blk + 1024 * G + ((t * 4 + i) * G) * 8);
     }
+}
+template <int G> DEV void kv4_fetch_v(uint32_t (&vc)[2 * G], uint32_t (&vs)[2 * G + 2 * (G & 1)], const uint8_t* blk, int m, int i) {
 #pragma unroll
     for (int p = 0; p < G / 2; ++p) {   // 64 dims: four neighbouring ones a lane
         const u32x4 w = ld16(blk + 512 * G + (i * 32 * G + 64 * p + 4 * m) * 4), s = ld16(blk + 1088 * G + (i * G + 2 * p + (m >> 3)) * 16);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { r.vc[4 * p + j] = w[j]; r.vs[4 * p + j] = s[j]; }
+        for (int j = 0; j < 4; ++j) { vc[4 * p + j] = w[j]; vs[4 * p + j] = s[j]; }
     }
     if constexpr (G & 1) {              // 32 dims: two a lane
         const u32x2 w = ld8(blk + 512 * G + (i * 32 * G + 32 * (G - 1) + 2 * m) * 4);
         const u32x4 s = ld16(blk + 1088 * G + (i * G + G - 1) * 16);
-        r.vc[2 * G - 2] = w[0]; r.vc[2 * G - 1] = w[1];
+        vc[2 * G - 2] = w[0]; vc[2 * G - 1] = w[1];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) r.vs[2 * (G - 1) + j] = s[j];
+        for (int j = 0; j < 4; ++j) vs[2 * (G - 1) + j] = s[j];
     }
 }
 // row `row` of the tile, `dim` of the head that register r of dim tile `j` holds for quad i
@@ -333,161 +496,179 @@ template <int G> DEV int kv4_dim(int j, int i, int r) {
     return j < 4 * (G / 2) ? 64 * (j / 4) + 16 * i + 4 * r + (j & 3) : 32 * (G - 1) + 8 * i + 2 * r + (j & 1);
 }
 
-template <int G, int NT> __global__ void __launch_bounds__(256) kv4_decode_kernel(const Kv4Attn a) {
-    constexpr int W = 4, DP = 32 * G, PITCH = DP + 4;
+template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 : G * NT <= 4 ? 3 : 2) kv4_decode_kernel(const Kv4Attn a) {
+    constexpr int W = 4, DP = 32 * G, PITCH = DP + 4, ROWS = 16 * NT;
     CT_DYN_SMEM(smem);
     float* part = (float*)smem;                       // [wave][row][PITCH] of one row tile
-    float* stat = part + W * 16 * PITCH;              // [wave][16 NT][2]: maximum, sum
+    float* stat = part + W * 16 * PITCH;              // [wave][ROWS][2]: maximum, sum
     const Kv4Cache& c = a.c;
-    const int lane = lane_id(), w = wave_id(), m = lane & 15, i = lane >> 4;
-    const int pairs = c.n_seq * c.n_head_kv, id = (int)blockIdx.x;
-    const int pair = id % pairs, rest = id / pairs, split = rest % a.nsplit, tile = rest / a.nsplit;
-    const int b = pair / c.n_head_kv, kvh = pair % c.n_head_kv;
-    const Kv4Range rg = kv4_range(a, b, tile, 16 * NT);
-    if (rg.n_rows <= 0 || (split >= rg.parts && split > 0)) return;
-    const int row0 = tile * 16 * NT;
+    const int w = uniform_int(wave_id());
+    // this workgroup's share [x, x_end) of the line; without a split a workgroup is one unit
+    int x = 0, x_end = 1, seq_begin = 0;
+    int b, in_seq;                                    // the unit's sequence, its index there
+    if (a.nsplit > 1) {
+        const Kv4Line line = kv4_line(a, ROWS, 0);
+        if ((long long)blockIdx.x * line.per >= line.all) return;
+        x = (int)blockIdx.x * line.per;
+        x_end = line.all - x < line.per ? line.all : x + line.per;
+        b = kv4_find(a, ROWS, x, seq_begin);
+        in_seq = 0;
+    } else {
+        const int per_seq = c.n_head_kv * a.tiles;
+        b = uniform_int((int)blockIdx.x / per_seq);
+        in_seq = (int)blockIdx.x - b * per_seq;
+    }
+  while (x < x_end) {
+    const int lane = kv4_anew(lane_id()), m = lane & 15, i = lane >> 4;
+    int lo, hi, len;
+    kv4_seq(c, b, lo, hi, len);
+    const int nq = hi - lo, nb = kv4_unit_blocks(a, nq, len), tiles = kv4_tiles(a, nq, ROWS);
+    int begin = 0, end = nb;
+    if (a.nsplit > 1) {
+        const int unit = nb + kUnitCost;
+        if (nb == 0 || x - seq_begin >= unit * tiles * c.n_head_kv) {   // on to the next sequence
+            seq_begin += nb == 0 ? 0 : unit * tiles * c.n_head_kv;
+            ++b;
+            continue;
+        }
+        in_seq = uniform_int((x - seq_begin) / unit);
+        const int at = x - seq_begin - in_seq * unit;
+        begin = at < kUnitCost ? 0 : at - kUnitCost;
+        end = x_end - x < unit - at ? at + x_end - x - kUnitCost : nb;
+        x += unit - at < x_end - x ? unit - at : x_end - x;
+        if (end <= begin) continue;                                     // the share ends before the unit's first block
+    } else {
+        x = x_end;
+        if (in_seq >= tiles * c.n_head_kv) return;
+    }
+    const int kvh = uniform_int(in_seq / tiles), tile = in_seq - kvh * tiles, row0 = tile * ROWS, n_rows = nq * a.rep - row0 < ROWS ? nq * a.rep - row0 : ROWS;
+    const bool whole = begin == 0 && end == nb;
 
     u32x4 q[NT][G];
-    float cq[NT][G], sc2[NT], mx[NT], sum[NT];
+    f32x4 cq[NT][G];
+    float sc2[NT], mx[NT], sum[NT];
     int lim[NT];
     f32x4 O[NT][2 * G];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int r = row0 + 16 * n + m;
-        const bool on = 16 * n + m < rg.n_rows;
+        const bool on = 16 * n + m < n_rows;
         const int tok = on ? r / a.rep : 0;
-        lim[n] = on ? rg.len - rg.nq + tok + 1 : 0;
-        const long long at = (long long)(rg.lo + tok) * a.q.row + (long long)(kvh * a.rep + (on ? r % a.rep : 0)) * a.q.head;
-        float x[G][8], big = 0.0f;
+        lim[n] = on ? len - nq + tok + 1 : 0;
+        const long long at = (long long)(lo + tok) * a.q.row + (long long)(kvh * a.rep + (on ? r - tok * a.rep : 0)) * a.q.head;
+        const float down = kv4_query<G>(q[n], a.q, at, 8 * i, 32, c.head_dim, on, [](float v) { v = fmaxf(v, lane_xor16(v)); return fmaxf(v, lane_xor32(v)); });
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const int d0 = 32 * g + 8 * i;
-            if (on && d0 < c.head_dim) kv4_load8(x[g], a.q, at + d0);
-            else for (int j = 0; j < 8; ++j) x[g][j] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[g][j]));
-        }
-        // Rows that f16 may not hold (bf16, f32) are scaled by a power of two that brings the largest value into [1, 2); bf16 stays exact but for values below
-        // 2^-17 of the row's largest.
-        float up = 1.0f, down = 1.0f;
-        if (a.q.type != KV4_F16) {
-            big = fmaxf(big, lane_xor16(big));
-            big = fmaxf(big, lane_xor32(big));
-            const int e = (int)((bits_of(big) >> 23) & 255u);
-            if (e > 0 && e < 254) { up = float_of((uint32_t)(254 - e) << 23); down = float_of((uint32_t)e << 23); }
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            float s = 0.0f;
-            uint32_t h[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                h[j] = kv4_cvt2(x[g][2 * j] * up, x[g][2 * j + 1] * up);
-                s += f16_bits_to_f32((uint16_t)(h[j] & 0xFFFFu));
-                s += f16_bits_to_f32((uint16_t)(h[j] >> 16));
-            }
-            s += lane_xor16(s);
-            s += lane_xor32(s);
-            cq[n][g] = s * (-8.0f / 16777216.0f);
-            q[n][g] = u32x4_of(h[0], h[1], h[2], h[3]);
-        }
+        for (int g = 0; g < G; ++g)   // -8 sum(Q) of the group in every row of the product: A all -8 (f16 bits 0x8008: -8 * 2^-24, as the codes are)
+            cq[n][g] = mfma_f16_16x16x32(u32x4_of(0x80088008u, 0x80088008u, 0x80088008u, 0x80088008u), q[n][g], f32x4_splat(0.0f));
         sc2[n] = a.scale * 1.44269504088896f * 16777216.0f * down;
         mx[n] = -INFINITY;
         sum[n] = 0.0f;
 #pragma unroll
         for (int j = 0; j < 2 * G; ++j) O[n][j] = f32x4_splat(0.0f);
     }
-    const int free_lim = rg.len - rg.nq + rg.first_tok + 1;   // every row of the tile sees the positions below
+    const int free_lim = len - nq + row0 / a.rep + 1;   // every row of the tile sees the positions below
 
-    const int end = (split + 1) * rg.per < rg.nb ? (split + 1) * rg.per : rg.nb;
-    auto compute = [&](const Kv4Raw<G>& r, int blk) {
-        const int p0 = blk * 32;
-        const bool edge = p0 + 32 > free_lim || p0 + 32 > rg.len;
-        u32x4 P[NT];
+    uint32_t kc[2][G], ks[2][2 * G], vc[2 * G], vs[2 * G + 2 * (G & 1)];
+    int blk = begin + w;
+    if (c.n_pages <= 0) end = begin;
+    // Loads are never conditional (a wait for V would have to count K's as not issued, and wait for them too): where there is no block, the pool's first is read
+    // and everything in it masked.
+    bool here = false;
+    int pid = -1;
+    if (blk < end) {
+        const uint8_t* p = kv4_in_page(c, kv4_page_of(c, b, blk), kvh, blk);
+        here = p != nullptr;
+        if (blk + W < end) pid = kv4_page_of(c, b, blk + W);
+        p = here ? p : c.pages;
+        kv4_fetch_k<G>(kc, ks, p, m, i);
+        kv4_fetch_v<G>(vc, vs, p, m, i);
+    }
+    for (; blk < end; blk += W) {
+        const int pid2 = blk + 2 * W < end ? kv4_page_of(c, b, blk + 2 * W) : -1;
+        const uint8_t* nxt = kv4_in_page(c, pid, kvh, blk + W);
+        const bool next_here = nxt != nullptr;
+        nxt = next_here ? nxt : c.pages;
+        const int p0 = blk * 32, there = here ? len : 0;   // tokens from `there` on are not there
+        float s[NT][2][4];
+        {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float s[2][4];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const uint32_t k = r.kc[t][g], M = 0x000F000Fu;
-                    const f32x4 acc = mfma_f16_16x16x32(u32x4_of(k & M, (k >> 4) & M, (k >> 8) & M, (k >> 12) & M), q[n][g], f32x4_splat(cq[n][g]));
+                    const uint32_t k = kc[t][g], M = 0x000F000Fu;
+                    const u32x4 kf = u32x4_of(k & M, (k >> 4) & M, (k >> 8) & M, (k >> 12) & M);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t d2 = r.ks[t][2 * g + e / 2];
-                        const float d = f16_bits_to_f32((uint16_t)(e & 1 ? d2 >> 16 : d2 & 0xFFFFu));
-                        s[t][e] = g == 0 ? d * acc[e] : fmaf(d, acc[e], s[t][e]);
+                    for (int n = 0; n < NT; ++n) {
+                        const f32x4 acc = mfma_f16_16x16x32(kf, q[n][g], cq[n][g]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t d2 = ks[t][2 * g + e / 2];
+                            const float d = f16_bits_to_f32((uint16_t)(e & 1 ? d2 >> 16 : d2 & 0xFFFFu));
+                            s[n][t][e] = g == 0 ? d * acc[e] : fmaf(d, acc[e], s[n][t][e]);
+                        }
                     }
                 }
-            }
-            float top = -INFINITY;
+        }
+        kv4_fetch_k<G>(kc, ks, nxt, m, i);
+        {
+            const bool edge = p0 + 32 > free_lim || p0 + 32 > there;
+            u32x4 P[NT];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int n = 0; n < NT; ++n) {
+                float top = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[t][e] *= sc2[n];
-                    if (edge && p0 + 16 * t + 4 * i + e >= lim[n]) s[t][e] = -INFINITY;
-                    top = fmaxf(top, s[t][e]);
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[n][t][e] *= sc2[n];
+                        if (edge && (p0 + 16 * t + 4 * i + e >= lim[n] || !here)) s[n][t][e] = -INFINITY;
+                        top = fmaxf(top, s[n][t][e]);
+                    }
+                if (__ballot(top > mx[n] + 8.0f)) {   // (also the first block: -inf + 8)
+                    top = fmaxf(top, lane_xor16(top));
+                    top = fmaxf(top, lane_xor32(top));
+                    const float now = fmaxf(mx[n], top);
+                    const float f = now == -INFINITY ? 1.0f : exp2_fast(mx[n] - now);
+                    mx[n] = now;
+                    sum[n] *= f;
+#pragma unroll
+                    for (int j = 0; j < 2 * G; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) O[n][j][e] *= f;
                 }
-            if (__ballot(top > mx[n] + 8.0f)) {   // (also the first block: -inf + 8)
-                top = fmaxf(top, lane_xor16(top));
-                top = fmaxf(top, lane_xor32(top));
-                const float now = fmaxf(mx[n], top);
-                const float f = now == -INFINITY ? 1.0f : exp2_fast(mx[n] - now);
-                mx[n] = now;
-                sum[n] *= f;
+                const float base = mx[n] == -INFINITY ? 0.0f : mx[n];
+                uint32_t pk[4];
 #pragma unroll
-                for (int j = 0; j < 2 * G; ++j)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) O[n][j][e] *= f;
+                    for (int e = 0; e < 4; e += 2) {
+                        const float x = exp2_fast(s[n][t][e] - base), y = exp2_fast(s[n][t][e + 1] - base);
+                        sum[n] += x;
+                        sum[n] += y;
+                        pk[2 * t + e / 2] = kv4_cvt2(x, y);   // the probabilities as halves: 2^-12 of each, independent of one another
+                    }
+                P[n] = u32x4_of(pk[0], pk[1], pk[2], pk[3]);
             }
-            const float base = mx[n] == -INFINITY ? 0.0f : mx[n];
-            uint32_t pk[4];
+            if (p0 + 32 > there) {   // whatever the page holds past the sequence's end must not meet p = 0 as an infinity
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+                for (int p = 0; p < 4; ++p) {
+                    const int t0 = p0 + 16 * (p / 2) + 4 * i + 2 * (p & 1);
+                    const uint32_t keep = (t0 < there ? 0xFFFFu : 0u) | (t0 + 1 < there ? 0xFFFF0000u : 0u);
 #pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    const float x = exp2_fast(s[t][e] - base), y = exp2_fast(s[t][e + 1] - base);
-                    sum[n] += x;
-                    sum[n] += y;
-                    pk[2 * t + e / 2] = kv4_cvt2(x, y);   // the probabilities as halves: 2^-12 of each, independent of one another
+                    for (int j = 0; j < 2 * G + 2 * (G & 1); j += 4) vs[j + p] &= keep;
                 }
-            P[n] = u32x4_of(pk[0], pk[1], pk[2], pk[3]);
-        }
-        // tokens past the sequence's end: whatever the page holds there must not meet p = 0 as an infinity
-        uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-        if (p0 + 32 > rg.len) {
+            }
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const int t0 = p0 + 16 * (p / 2) + 4 * i + 2 * (p & 1);
-                keep[p] = (t0 < rg.len ? 0xFFFFu : 0u) | (t0 + 1 < rg.len ? 0xFFFF0000u : 0u);
+            for (int j = 0; j < 2 * G; ++j) {
+                const int s0 = j < 4 * (G / 2) ? 4 * (j / 4) : 2 * (G - 1);
+                const u32x4 v = kv4_values(vc[j], vs[s0], vs[s0 + 1], vs[s0 + 2], vs[s0 + 3]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) O[n][j] = mfma_f16_16x16x32(v, P[n], O[n][j]);
             }
         }
-#pragma unroll
-        for (int j = 0; j < 2 * G; ++j) {
-            const int s0 = j < 4 * (G / 2) ? 4 * (j / 4) : 2 * (G - 1);
-            const u32x4 v = kv4_values(r.vc[j], r.vs[s0] & keep[0], r.vs[s0 + 1] & keep[1], r.vs[s0 + 2] & keep[2], r.vs[s0 + 3] & keep[3]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) O[n][j] = mfma_f16_16x16x32(v, P[n], O[n][j]);
-        }
-    };
-    {
-        Kv4Raw<G> r0, r1;
-        int blk = split * rg.per + w;
-        const uint8_t* p0 = blk < end ? kv4_block(c, b, kvh, uniform_int(blk)) : nullptr;
-        if (p0) kv4_fetch<G>(r0, p0, m, i);
-        while (blk < end) {
-            const uint8_t* p1 = blk + W < end ? kv4_block(c, b, kvh, uniform_int(blk + W)) : nullptr;
-            if (p1) kv4_fetch<G>(r1, p1, m, i);
-            if (p0) compute(r0, blk);
-            blk += W;
-            if (blk >= end) break;
-            p0 = blk + W < end ? kv4_block(c, b, kvh, uniform_int(blk + W)) : nullptr;
-            if (p0) kv4_fetch<G>(r0, p0, m, i);
-            if (p1) compute(r1, blk);
-            blk += W;
-        }
+        kv4_fetch_v<G>(vc, vs, nxt, m, i);
+        here = next_here;
+        pid = pid2;
     }
     // the waves' results meet in LDS, in wave order
 #pragma unroll
@@ -496,8 +677,7 @@ template <int G, int NT> __global__ void __launch_bounds__(256) kv4_decode_kerne
         sum[n] += lane_xor32(sum[n]);
         if (i == 0) { stat[(w * 16 * NT + 16 * n + m) * 2] = mx[n]; stat[(w * 16 * NT + 16 * n + m) * 2 + 1] = sum[n]; }
     }
-    const bool whole = rg.parts <= 1;
-    float* out = a.ws + ((long long)(tile * (long long)pairs + pair) * a.nsplit + split) * (16 * NT) * (c.head_dim + 2);
+    float* out = a.ws + ((long long)blockIdx.x * 2 + (begin == 0)) * ROWS * (c.head_dim + 2);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         if (n) __syncthreads();
@@ -506,9 +686,9 @@ template <int G, int NT> __global__ void __launch_bounds__(256) kv4_decode_kerne
 #pragma unroll
             for (int e = 0; e < 4; ++e) part[(w * 16 + m) * PITCH + kv4_dim<G>(j, i, e)] = O[n][j][e];
         __syncthreads();
-        for (int it = (int)threadIdx.x; it < 16 * DP; it += 64 * W) {
+        for (int it = 64 * w + lane; it < 16 * DP; it += 64 * W) {
             const int row = it / DP, dim = it % DP;
-            if (16 * n + row >= rg.n_rows || dim >= c.head_dim) continue;
+            if (16 * n + row >= n_rows || dim >= c.head_dim) continue;
             float M = -INFINITY, L = 0.0f, v = 0.0f;
 #pragma unroll
             for (int k = 0; k < W; ++k) M = fmaxf(M, stat[(k * 16 * NT + 16 * n + row) * 2]);
@@ -521,7 +701,7 @@ template <int G, int NT> __global__ void __launch_bounds__(256) kv4_decode_kerne
             }
             if (whole) {
                 const int r = row0 + 16 * n + row;
-                kv4_store_any(a.out, (long long)(rg.lo + r / a.rep) * a.o_row + (long long)(kvh * a.rep + r % a.rep) * a.o_head + dim, a.out_type, L == 0.0f ? 0.0f : v / L);
+                kv4_store_any(a.out, (long long)(lo + r / a.rep) * a.o_row + (long long)(kvh * a.rep + r % a.rep) * a.o_head + dim, a.out_type, L == 0.0f ? 0.0f : v / L);
             } else {
                 float* o = out + (16 * n + row) * (c.head_dim + 2);
                 o[2 + dim] = v;
@@ -529,48 +709,94 @@ template <int G, int NT> __global__ void __launch_bounds__(256) kv4_decode_kerne
             }
         }
     }
+    if (a.nsplit > 1) __syncthreads();   // LDS is the next unit's
+  }
 }
 
-// The parts of a row joined: one wave per (row, head).
-template <int NR> __global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Attn a, int tile_rows) {
+// The parts of a row joined: a workgroup of W waves per (row, head); a wave takes every W-th part, four at a time, two dims a lane, with a maximum of its own.
+// LINE: parts are shares' ends (kv4_decode_kernel), else the splits of kv4_prompt_kernel.
+template <int NR, bool LINE, int W> __global__ void __launch_bounds__(64 * W) kv4_join_kernel(const Kv4Attn a, int tile_rows) {
+    __shared__ float acc[W][128 * NR], stat[W][2];
     const Kv4Cache& c = a.c;
-    const int lane = lane_id(), item = (int)blockIdx.x * 4 + wave_id();
-    const int row = item / a.n_head, head = item % a.n_head;
-    if (row >= c.total) return;
+    const int lane = lane_id(), w = uniform_int(wave_id()), row = (int)blockIdx.x / a.n_head, head = (int)blockIdx.x % a.n_head;
     int b = 0;
-    if (c.cu) {   // the last sequence that begins at or before the row
-        int lo = 0, hi = c.n_seq;
-        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (c.cu[mid] <= row) lo = mid; else hi = mid; }
-        b = lo;
-        if (row < c.cu[b] || row >= c.cu[b + 1]) return;   // behind the last sequence
+    if (c.cu) {   // the last sequence that begins at or before the row (their number, less one)
+        int n = 0;
+        for (int k = 0; k < c.n_seq; k += 64) n += __popcll(__ballot(k + lane < c.n_seq && c.cu[k + lane] <= row));
+        b = uniform_int(n) - 1;
+        if (b < 0 || row >= c.cu[b + 1]) return;   // behind the last sequence
     }
-    const int kvh = head / a.rep, r = (row - (c.cu ? c.cu[b] : 0)) * a.rep + head % a.rep, tile = r / tile_rows;
-    if (tile >= a.tiles) return;
-    const Kv4Range rg = kv4_range(a, b, tile, tile_rows);
-    if (rg.parts <= 1) return;
-    const long long pairs = (long long)c.n_seq * c.n_head_kv, step = (long long)tile_rows * (c.head_dim + 2);
-    const float* in = a.ws + ((long long)(tile * pairs + (long long)b * c.n_head_kv + kvh) * a.nsplit) * step + (long long)(r % tile_rows) * (c.head_dim + 2);
-    float M = -INFINITY;
-    for (int s = lane; s < rg.parts; s += 64) M = fmaxf(M, in[s * step]);
-    M = wave_max(M);
-    const float base = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f, o[NR];
-    for (int j = 0; j < NR; ++j) o[j] = 0.0f;
-    for (int s0 = 0; s0 < rg.parts; s0 += 64) {
-        const int s = s0 + lane;
-        const float f = s < rg.parts ? exp2_fast(in[s * step] - base) : 0.0f;
-        L += s < rg.parts ? f * in[s * step + 1] : 0.0f;
-        const int n = rg.parts - s0 < 64 ? rg.parts - s0 : 64;
-        for (int k = 0; k < n; ++k) {
-            const float fk = __shfl(f, k);
+    int lo, hi, len;
+    kv4_seq(c, b, lo, hi, len);
+    const int kvh = head / a.rep, r = (row - lo) * a.rep + head % a.rep, tile = r / tile_rows, dim = c.head_dim;
+    const long long step = (long long)tile_rows * (dim + 2);
+    int parts;
+    const float *in, *in0;   // part 0 and the others' origin
+    if constexpr (LINE) {
+        const Kv4Line line = kv4_line(a, tile_rows, b);
+        const int nb = kv4_unit_blocks(a, hi - lo, len), tiles = kv4_tiles(a, hi - lo, tile_rows);
+        if (tile >= tiles) return;
+        const int x = line.before + (kvh * tiles + tile) * (nb + kUnitCost) + kUnitCost, s0 = x / line.per;   // the unit's first block
+        parts = (x + nb - 1) / line.per - s0 + 1;
+        in0 = a.ws + (2ll * s0 + 1) * step;
+        in = a.ws + 2ll * s0 * step;
+    } else {
+        if (tile >= a.tiles) return;
+        const Kv4Range rg = kv4_range(a, b, tile, tile_rows, kv4_part(a));
+        parts = rg.parts;
+        in0 = in = a.ws + ((long long)(tile * ((long long)c.n_seq * c.n_head_kv) + (long long)b * c.n_head_kv + kvh) * a.nsplit) * step;
+    }
+    if (parts <= 1) return;
+    const long long at_row = (long long)(r % tile_rows) * (dim + 2);
+    float M = -INFINITY, L = 0.0f, o[2 * NR];
 #pragma unroll
-            for (int j = 0; j < NR; ++j) if (lane + 64 * j < c.head_dim) o[j] += fk * in[(s0 + k) * step + 2 + lane + 64 * j];
+    for (int j = 0; j < 2 * NR; ++j) o[j] = 0.0f;
+    for (int s0 = w; s0 < parts; s0 += 4 * W) {
+        float pm[4], pl[4], now = M;
+        u32x2 v[4][NR];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int s = s0 + W * k;
+            const float* p = (s == 0 || s >= parts ? in0 : in + (LINE ? 2 : 1) * s * step) + at_row;
+            pm[k] = p[0];
+            pl[k] = p[1];
+#pragma unroll
+            for (int j = 0; j < NR; ++j) v[k][j] = ld8(p + 2 + (2 * lane + 128 * j < dim ? 2 * lane + 128 * j : 0));
+            if (s >= parts) pm[k] = -INFINITY;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) now = fmaxf(now, pm[k]);
+        const float base = now == -INFINITY ? 0.0f : now, f = exp2_fast(M - base);
+        M = now;
+        L *= f;
+#pragma unroll
+        for (int j = 0; j < 2 * NR; ++j) o[j] *= f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (s0 + W * k >= parts) continue;
+            const float g = exp2_fast(pm[k] - base);
+            L += g * pl[k];
+#pragma unroll
+            for (int j = 0; j < NR; ++j) { o[2 * j] += g * float_of(v[k][j][0]); o[2 * j + 1] += g * float_of(v[k][j][1]); }
         }
     }
-    L = wave_sum(L);
-    const long long at = (long long)row * a.o_row + (long long)head * a.o_head;
 #pragma unroll
-    for (int j = 0; j < NR; ++j) if (lane + 64 * j < c.head_dim) kv4_store_any(a.out, at + lane + 64 * j, a.out_type, L == 0.0f ? 0.0f : o[j] / L);
+    for (int j = 0; j < NR; ++j) { acc[w][128 * j + 2 * lane] = o[2 * j]; acc[w][128 * j + 2 * lane + 1] = o[2 * j + 1]; }
+    if (lane == 0) { stat[w][0] = M; stat[w][1] = L; }
+    __syncthreads();
+    for (int d = (int)threadIdx.x; d < dim; d += 64 * W) {
+        float top = -INFINITY, sum = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) top = fmaxf(top, stat[k][0]);
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const float f = exp2_fast(stat[k][0] - base);
+            sum += f * stat[k][1];
+            v += f * acc[k][d];
+        }
+        kv4_store_any(a.out, (long long)row * a.o_row + (long long)head * a.o_head + d, a.out_type, sum == 0.0f ? 0.0f : v / sum);
+    }
 }
 
 // Many rows (a prompt, a chunk of one): a workgroup of four waves takes 128 rows, a wave 32 of them; the blocks pass through LDS as halves, two at a time, so that a
@@ -593,6 +819,7 @@ DEV u32x4 lds_ld16(const unsigned char* p) { return *(const u32x4*)p; }
 template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prompt_kernel(const Kv4Attn a) {
     typedef Kv4Lds<G> L;
     CT_DYN_SMEM(smem);
+    __shared__ int here[4];   // [buffer][block]: the block is there
     const Kv4Cache& c = a.c;
     const int tid = (int)threadIdx.x, lane = lane_id(), w = wave_id(), n = lane & 31, h = lane >> 5;
     // workgroup -> (pair, split, tile): ids that are equal modulo 8 share an XCD
@@ -601,7 +828,7 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
     if (pair >= pairs) return;
     const int split = slot % a.nsplit, tile = a.tiles - 1 - slot / a.nsplit;
     const int b = pair / c.n_head_kv, kvh = pair % c.n_head_kv;
-    const Kv4Range rg = kv4_range(a, b, tile, 128);
+    const Kv4Range rg = kv4_range(a, b, tile, 128, kv4_part(a));
     if (rg.n_rows <= 0 || (split >= rg.parts && split > 0)) return;
 
     const int local = 32 * w + n, r = tile * 128 + local;
@@ -609,33 +836,9 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
     const int tok = on ? r / a.rep : 0, head = kvh * a.rep + (on ? r % a.rep : 0);
     const int lim = on ? rg.len - rg.nq + tok + 1 : 0;
     u32x4 q[2 * G];
-    float sc2;
-    {
-        const long long at = (long long)(rg.lo + tok) * a.q.row + (long long)head * a.q.head;
-        float big = 0.0f, up = 1.0f, down = 1.0f;
-        if (a.q.type != KV4_F16) {   // as in kv4_decode_kernel: a power of two for the row
-#pragma unroll
-            for (int k = 0; k < 2 * G; ++k) {
-                float x[8];
-                if (on && 16 * k + 8 * h < c.head_dim) {
-                    kv4_load8(x, a.q, at + 16 * k + 8 * h);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[j]));
-                }
-            }
-            big = fmaxf(big, lane_xor32(big));
-            const int e = (int)((bits_of(big) >> 23) & 255u);
-            if (e > 0 && e < 254) { up = float_of((uint32_t)(254 - e) << 23); down = float_of((uint32_t)e << 23); }
-        }
-#pragma unroll
-        for (int k = 0; k < 2 * G; ++k) {
-            float x[8];
-            if (on && 16 * k + 8 * h < c.head_dim) kv4_load8(x, a.q, at + 16 * k + 8 * h);
-            else for (int j = 0; j < 8; ++j) x[j] = 0.0f;
-            q[k] = u32x4_of(kv4_cvt2(x[0] * up, x[1] * up), kv4_cvt2(x[2] * up, x[3] * up), kv4_cvt2(x[4] * up, x[5] * up), kv4_cvt2(x[6] * up, x[7] * up));
-        }
-        sc2 = a.scale * 1.44269504088896f * down;
-    }
+    const float down = kv4_query<2 * G>(q, a.q, (long long)(rg.lo + tok) * a.q.row + (long long)head * a.q.head, 8 * h, 16, c.head_dim, on,
+                                        [](float v) { return fmaxf(v, lane_xor32(v)); });
+    const float sc2 = a.scale * 1.44269504088896f * down;
     float mx = -INFINITY, sum = 0.0f;
     f32x16 O[G];
 #pragma unroll
@@ -651,9 +854,10 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
     const int sb = tid >> 7, st = (tid >> 2) & 31, si = tid & 3, sd = tid & 31, ve = (tid >> 5) & 3;
     uint32_t kc[G], ks[G], vc[G], vs[G][4];
     bool got = false;
+    int pid = -1;
+    auto look_up = [&](int blk) { pid = blk + sb < end ? kv4_page_of(c, b, uniform_int(blk + sb)) : -1; };   // (sb is the same for a whole wave)
     auto fetch = [&](int blk) {
-        const int bb = blk + sb;
-        const uint8_t* p = bb < end ? kv4_block(c, b, kvh, bb) : nullptr;
+        const uint8_t* p = kv4_in_page(c, pid, kvh, blk + sb);
         got = p != nullptr;
         if (!got) return;
         kv4_ldw<G>(kc, p + ((st * 4 + si) * G) * 4);
@@ -678,7 +882,7 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
                 keep[p] = (t0 < rg.len ? 0xFFFFu : 0u) | (t0 + 1 < rg.len ? 0xFFFF0000u : 0u);
             }
         }
-        // an absent block: K is NaN only where it is masked anyway (see `gone`), V is 0
+        if ((tid & 127) == 0) here[buf * 2 + sb] = got;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const uint32_t s = got ? ks[g] | (ks[g] << 16) : 0u;
@@ -693,15 +897,13 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
         if (p0 >= wend) return;
         f32x16 S[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const unsigned char* kb = smem + (buf * 2 + k) * L::BLK;
+        for (int g = 0; g < 2 * G; ++g)   // two independent sums
 #pragma unroll
-            for (int g = 0; g < 2 * G; ++g) {
-                const u32x4 kf = lds_ld16(kb + (2 * g + h) * L::KC + tk * 16);
+            for (int k = 0; k < 2; ++k) {
+                const u32x4 kf = lds_ld16(smem + (buf * 2 + k) * L::BLK + (2 * g + h) * L::KC + tk * 16);
                 S[k] = g == 0 ? mfma_f16_32x32x16(kf, q[g]) : mfma_f16_32x32x16_acc(kf, q[g], S[k]);
             }
-        }
-        const bool gone0 = !kv4_block(c, b, kvh, uniform_int(blk)), gone1 = blk + 1 >= end || !kv4_block(c, b, kvh, uniform_int(blk + 1));
+        const bool gone0 = !here[buf * 2], gone1 = !here[buf * 2 + 1];
         const bool edge = p0 + 64 > wfree || gone0 || gone1;
         float top = -INFINITY;
 #pragma unroll
@@ -747,13 +949,15 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
         }
     };
     if (begin < end) {
+        look_up(begin);
         fetch(begin);
+        look_up(begin + 2);
         stage(begin, 0);
         int buf = 0;
         for (int blk = begin; blk < end; blk += 2, buf ^= 1) {
             __syncthreads();
             const bool more = blk + 2 < end;
-            if (more) fetch(blk + 2);
+            if (more) { fetch(blk + 2); look_up(blk + 4); }
             compute(blk, buf);
             if (more) stage(blk + 2, buf ^ 1);
         }

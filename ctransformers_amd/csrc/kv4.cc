@@ -68,6 +68,8 @@ static bool append_grid(Kv4Append& a, int max_rows, dim3& grid, const char*& err
     const long long x = (long long)a.blocks * c.n_seq;
     if (x > 0x7FFFFFFF) { err = "too many rows times sequences for one call"; return false; }
     grid = dim3((unsigned)x, (unsigned)c.n_head_kv);
+    rows_vec(a.k);
+    rows_vec(a.v);
     return true;
 }
 
@@ -75,8 +77,6 @@ bool kv4_append(Kv4Append& a, int max_rows, hipStream_t stream, const char*& err
     dim3 grid;
     if (a.c.total == 0 || a.c.n_seq == 0 || a.c.n_pages == 0 || max_rows <= 0) return true;
     if (!append_grid(a, max_rows, grid, err)) return false;
-    rows_vec(a.k);
-    rows_vec(a.v);
     KV4_BY_GROUPS(a.c.groups, CT_LAUNCH(kv4_append_kernel<G>, grid, dim3(256), stream, a);)
     return launched(err);
 }
@@ -95,8 +95,20 @@ static int tile_rows(const Kv4Attn& a, long long rows) {
     if (rows <= 32 && a.c.groups <= 4) return 32;
     return 128;
 }
-// Workgroups that one call should have at least: a chip full of them twice over.
-constexpr long long kWantGroups = 1024;
+static int chip_cus() {   // of the current device; asked for once per device
+    static int n_cu[16] = {};
+    int d = 0, n = 0;
+#ifndef CT_EMU
+    if (hipGetDevice(&d) != hipSuccess || d < 0 || d > 15) d = 0;
+#endif
+    if (!n_cu[d]) n_cu[d] = hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, d) == hipSuccess && n > 0 ? n : 256;
+    return n_cu[d];
+}
+// workgroups of a line of at most `units` x `blocks` blocks
+static long long shares(const Kv4Attn& a, long long units, long long blocks) {
+    const long long most = units * (blocks + kUnitCost) / (a.min_blocks + kUnitCost) + 1;   // (a share is no shorter than that)
+    return most < a.want_parts ? most : a.want_parts;
+}
 
 long long kv4_attention_plan(Kv4Attn& a, int max_rows) {
     const Kv4Cache& c = a.c;
@@ -105,25 +117,44 @@ long long kv4_attention_plan(Kv4Attn& a, int max_rows) {
     const long long rows = (long long)max_rows * a.rep;
     const int tr = tile_rows(a, rows);
     a.tiles = (int)((rows + tr - 1) / tr);
-    // The keys of a tile are split over workgroups until the chip is full, as far as the table's width allows parts of a useful size; how many parts a sequence
-    // really has follows from its own length, on the device.
-    const long long blocks = (long long)c.table_width << c.bshift, groups = (long long)c.n_seq * c.n_head_kv * a.tiles;
-    a.min_blocks = tr == 128 ? 16 : 8;
-    long long split = groups ? kWantGroups / groups : 1;
+    // The grid is for the longest sequences that the table has room for: how long they are is known on the device only.
+    const long long blocks = (long long)c.table_width << c.bshift, units = (long long)c.n_seq * c.n_head_kv * a.tiles;
+    const int cus = chip_cus();
+    if (tr < 128) {   // shares of the line (kv4_decode_kernel): as many as are resident at once; one unit a workgroup where a unit is no longer than the least share
+        const int g = c.groups * tr / 16;
+        a.min_blocks = 8;
+        a.want_parts = cus * (g <= 2 ? 4 : g <= 4 ? 3 : 2);
+        a.nsplit = blocks <= a.min_blocks ? 1 : 2;
+        return a.nsplit > 1 ? 2ll * shares(a, units, blocks) * tr * (c.head_dim + 2) : 0;
+    }
+    // Where there are too few tiles to fill the chip their keys are split, in parts that come out at about two a CU over the whole call (kv4_part).
+    a.min_blocks = 16;
+    a.want_parts = 2 * cus;
+    long long split = units ? a.want_parts / units : 1;
     const long long most = (blocks + a.min_blocks - 1) / a.min_blocks;
     if (split > most) split = most;
     if (split > 256) split = 256;
     if (split < 1) split = 1;
     a.nsplit = (int)split;
-    return split > 1 ? groups * split * tr * (c.head_dim + 2) : 0;
+    return split > 1 ? units * split * tr * (c.head_dim + 2) : 0;
 }
 
 template <int G, int NT> static void launch_decode(const Kv4Attn& a, hipStream_t stream) {
     constexpr size_t smem = (size_t)(4 * 16 * (32 * G + 4) + 4 * 16 * NT * 2) * 4;
     auto kfn = kv4_decode_kernel<G, NT>;
     KV4_OPTIN(kfn, smem);
-    const long long n = (long long)a.c.n_seq * a.c.n_head_kv * a.tiles * a.nsplit;
+    const long long units = (long long)a.c.n_seq * a.c.n_head_kv * a.tiles, n = a.nsplit > 1 ? shares(a, units, (long long)a.c.table_width << a.c.bshift) : units;
     CT_LAUNCH_DYN(kfn, dim3((unsigned)n), dim3(256), smem, stream, a);
+}
+
+template <int W> static void launch_join(const Kv4Attn& a, int tr, dim3 grid, hipStream_t stream) {
+    if (tr < 128) {
+        if (a.c.head_dim <= 128) CT_LAUNCH((kv4_join_kernel<1, true, W>), grid, dim3(64 * W), stream, a, tr);
+        else CT_LAUNCH((kv4_join_kernel<2, true, W>), grid, dim3(64 * W), stream, a, tr);
+    } else {
+        if (a.c.head_dim <= 128) CT_LAUNCH((kv4_join_kernel<1, false, W>), grid, dim3(64 * W), stream, a, tr);
+        else CT_LAUNCH((kv4_join_kernel<2, false, W>), grid, dim3(64 * W), stream, a, tr);
+    }
 }
 
 bool kv4_attention(Kv4Attn& a, int max_rows, long long ws_floats, hipStream_t stream, const char*& err) {
@@ -134,8 +165,9 @@ bool kv4_attention(Kv4Attn& a, int max_rows, long long ws_floats, hipStream_t st
     const long long want = kv4_attention_plan(a, max_rows);
     if (want > ws_floats || (want && !a.ws)) { err = "workspace too small"; return false; }
     const long long pairs = (long long)c.n_seq * c.n_head_kv, grid = ((pairs + 7) & ~7ll) * a.tiles * a.nsplit;
-    if (grid > 0x7FFFFFFF || (long long)c.total * a.n_head > 0x7FFFFFFF) { err = "too many rows times sequences for one call"; return false; }
     rows_vec(a.q);
+    if (pairs * a.tiles * (((long long)c.table_width << c.bshift) + kUnitCost) > 0x7FFFFFFF) { err = "a table with room for 2^31 blocks or more over all heads"; return false; }
+    if (grid > 0x7FFFFFFF || (long long)c.total * a.n_head > 0x7FFFFFFF) { err = "too many rows times sequences for one call"; return false; }
     const int tr = tile_rows(a, (long long)(max_rows > c.total ? c.total : max_rows) * a.rep);
     if (tr == 16) {
         KV4_BY_GROUPS(c.groups, (launch_decode<G, 1>(a, stream));)
@@ -155,11 +187,10 @@ bool kv4_attention(Kv4Attn& a, int max_rows, long long ws_floats, hipStream_t st
         })
     }
     if (a.nsplit > 1) {
-        const dim3 jg((unsigned)(((long long)c.total * a.n_head + 3) / 4));
-        const int nr = (c.head_dim + 63) / 64;
-        if (nr == 1) CT_LAUNCH(kv4_join_kernel<1>, jg, dim3(256), stream, a, tr);
-        else if (nr == 2) CT_LAUNCH(kv4_join_kernel<2>, jg, dim3(256), stream, a, tr);
-        else CT_LAUNCH(kv4_join_kernel<4>, jg, dim3(256), stream, a, tr);
+        const dim3 jg((unsigned)((long long)c.total * a.n_head));
+        // few rows: eight waves for each, their parts are many; many rows: a wave each, all of them resident at once
+        if ((long long)c.total * a.n_head <= 2048) launch_join<8>(a, tr, jg, stream);
+        else launch_join<1>(a, tr, jg, stream);
     }
     return launched(err);
 }

@@ -19,150 +19,140 @@ launched.  There is no CPU path: without the HIP library, or with tensors elsewh
 import ctypes
 import math
 import os
-from ctypes import POINTER, Structure, byref, c_float, c_int, c_longlong, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
+from struct import Struct
 
 import torch
 
 from .llm import find_library
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_INT = torch.int32
 
-
-class _Cache(Structure):
-    _fields_ = [("pages", c_void_p), ("table", c_void_p), ("lens", c_void_p), ("cu", c_void_p), ("page_stride", c_longlong), ("n_pages", c_int),
-                ("table_stride", c_int), ("table_width", c_int), ("n_seq", c_int), ("total", c_int), ("n_head_kv", c_int), ("head_dim", c_int),
-                ("page_tokens", c_int), ("max_rows", c_int)]
-
-
-class _Rows(Structure):
-    _fields_ = [("p", c_void_p), ("row", c_longlong), ("head", c_longlong), ("dim", c_longlong), ("type", c_int)]
-
-
-class _Tables(Structure):
-    _fields_ = [("table", c_void_p), ("lens", c_void_p), ("refs", c_void_p), ("table_out", c_void_p), ("lens_out", c_void_p), ("refs_out", c_void_p),
-                ("n_seq", c_int), ("width", c_int), ("n_pages", c_int), ("page_tokens", c_int)]
-
+# The C structures as packed bytes (a token step calls an operator per layer: building ctypes structures field by field costs more than the GPU's work at small sizes)
+CACHE = Struct("@4Pq9i4x")    # ctamd_kv4_cache
+ROWS = Struct("@P3qi4x")      # ctamd_rows
+TABLES = Struct("@6P4i")      # ctamd_kv_tables
 
 # name -> (restype, argtypes); the CPU test-suite checks include/ctransformers_amd_ops.h and the built library against this table
 ABI = {
-    "ctamd_ops_error": (ctypes.c_char_p, []),
+    "ctamd_ops_error": (c_char_p, []),
     "ctamd_ops_host_memory": (c_int, []),
     "ctamd_kv4_page_bytes": (c_longlong, [c_int, c_int, c_int]),
-    "ctamd_kv4_append": (c_int, [POINTER(_Cache), POINTER(_Rows), POINTER(_Rows), c_void_p]),
-    "ctamd_kv4_read": (c_int, [POINTER(_Cache), POINTER(_Rows), POINTER(_Rows), c_void_p]),
-    "ctamd_kv4_attention_ws": (c_longlong, [POINTER(_Cache), c_int]),
-    "ctamd_kv4_attention": (c_int, [POINTER(_Cache), c_int, POINTER(_Rows), POINTER(_Rows), c_float, c_void_p, c_longlong, c_void_p]),
-    "ctamd_kv_fork": (c_int, [POINTER(_Tables), c_void_p, c_int, c_void_p]),
+    "ctamd_kv4_append": (c_int, [c_char_p, c_char_p, c_char_p, c_void_p]),
+    "ctamd_kv4_read": (c_int, [c_char_p, c_char_p, c_char_p, c_void_p]),
+    "ctamd_kv4_attention_ws": (c_longlong, [c_char_p, c_int]),
+    "ctamd_kv4_attention": (c_int, [c_char_p, c_int, c_char_p, c_char_p, c_float, c_void_p, c_longlong, c_void_p]),
+    "ctamd_kv_fork": (c_int, [c_char_p, c_void_p, c_int, c_void_p]),
     "ctamd_kv_reserve_ws": (c_longlong, [c_int, c_int]),
-    "ctamd_kv_reserve": (c_int, [POINTER(_Tables), c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p]),
+    "ctamd_kv_reserve": (c_int, [c_char_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p]),
     "ctamd_kv_compact_ws": (c_longlong, [c_int]),
-    "ctamd_kv_compact": (c_int, [POINTER(_Tables), c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p]),
+    "ctamd_kv_compact": (c_int, [c_char_p, c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p]),
 }
 _lib = None
-_device = "cuda"
+_on_gpu = True
 
 
 def load(path=None):
     """Binds the library (`path`: another one than the package's).  Called by the first operator; returns the ctypes library."""
-    global _lib, _device
+    global _lib, _on_gpu
     lib = ctypes.CDLL(find_library(path))
     for name, (restype, argtypes) in ABI.items():
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = restype, argtypes
-    if not lib.ctamd_ops_host_memory() and os.path.exists("/proc/self/maps"):
+    on_gpu = not lib.ctamd_ops_host_memory()
+    if on_gpu and os.path.exists("/proc/self/maps"):
         with open("/proc/self/maps") as f:
             runtimes = {line.split()[-1] for line in f if "libamdhip64" in line}
         if len(runtimes) > 1:   # a stream of one runtime means nothing to the other
             raise RuntimeError("two HIP runtimes in this process (%s): import torch before the first model is loaded" % ", ".join(sorted(runtimes)))
-    _device = "cpu" if lib.ctamd_ops_host_memory() else "cuda"
-    _lib = lib
+    _lib, _on_gpu = lib, on_gpu
     return lib
 
 
-def _library():
-    return _lib if _lib is not None else load()
-
-
-def _call(code):
+def _launch(device, fn):
+    """fn(stream) with the tensors' device (its index) current, on that device's current stream."""
+    if device < 0:
+        code = fn(None)
+    elif device == torch.cuda.current_device():
+        code = fn(torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            code = fn(torch.cuda.current_stream(device).cuda_stream)
     if code:
         raise ValueError(_lib.ctamd_ops_error().decode())
 
 
-class _On:
-    """The tensors' device made current for a call, if it is not; `stream` is its current stream."""
-    __slots__ = ("guard", "stream")
-
-    def __init__(self, device):
-        self.guard = None
-        if device.type != "cuda":
-            self.stream = None
-            return
-        if device.index is not None and device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(device)
-            self.guard.__enter__()
-        self.stream = torch.cuda.current_stream().cuda_stream
-
-    def __enter__(self):
-        return self.stream
-
-    def __exit__(self, *what):
-        if self.guard is not None:
-            self.guard.__exit__(*what)
-
-
-def _ints(name, x, device, *shape):
-    if not isinstance(x, torch.Tensor) or x.dtype != torch.int32:
+def _ints(device, name, x, dims, rows=None):
+    """x: int32, `dims`-dimensional, entries adjacent, `rows` of them; returns its address."""
+    if not isinstance(x, torch.Tensor) or x.dtype is not _INT:
         raise TypeError("%s is an int32 tensor" % name)
-    if x.device != device:
-        raise ValueError("%s is on %s, not on %s" % (name, x.device, device))
-    if x.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, x.shape)):
-        raise ValueError("%s has shape %s" % (name, tuple(x.shape)))
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
+    if x.get_device() != device:
+        raise ValueError("%s is on %s, not on device %d" % (name, x.device, device))
+    shape = x.shape
+    if len(shape) != dims or (rows is not None and shape[0] != rows):
+        raise ValueError("%s has shape %s" % (name, tuple(shape)))
+    if x.stride()[-1] != 1 and shape[-1] > 1:
         raise ValueError("the entries of %s are not adjacent" % name)
+    return x.data_ptr()
 
 
-def _rows(name, x, device, shape=None):
-    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES:
+def _rows(device, name, x, shape=None):
+    t = _TYPES.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if t is None:
         raise TypeError("%s is a float16, bfloat16 or float32 tensor" % name)
-    if x.device != device:
-        raise ValueError("%s is on %s, not on %s" % (name, x.device, device))
-    if x.dim() != 3 or (shape is not None and tuple(x.shape) != tuple(shape)):
+    if x.get_device() != device:
+        raise ValueError("%s is on %s, not on device %d" % (name, x.device, device))
+    if len(x.shape) != 3 or (shape is not None and x.shape != shape):
         raise ValueError("%s has shape %s%s" % (name, tuple(x.shape), "" if shape is None else ", not %s" % (tuple(shape),)))
-    s = x.stride()
-    return _Rows(x.data_ptr(), s[0], s[1], s[2], _TYPES[x.dtype])
+    return ROWS.pack(x.data_ptr(), *x.stride(), t)
 
 
-def _cache(pages, table, lens, cu, total, n_head_kv, head_dim, page_tokens, max_rows):
-    _library()
-    if not isinstance(pages, torch.Tensor) or pages.dtype != torch.uint8:
+def _device_of(name, x):
+    if _lib is None:
+        load()
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("%s is a tensor" % name)
+    device = x.get_device()
+    if (device < 0) is _on_gpu:
+        raise ValueError("%s is on %s: the operators run on GPU memory only" % (name, x.device))
+    return device
+
+
+def _cache(device, pages, table, lens, cu, total, n_head_kv, head_dim, page_tokens, max_rows):
+    if pages.dtype is not torch.uint8:
         raise TypeError("pages is a uint8 tensor")
-    device = pages.device
-    if device.type != _device:
-        raise ValueError("pages is on %s: the operators run on GPU memory only" % device)
     width = _lib.ctamd_kv4_page_bytes(n_head_kv, head_dim, page_tokens)
     if not width:
         raise ValueError("sizes not supported: head_dim %s (a multiple of 8 up to 256), page_tokens %s (32, 64, 128 or 256), n_head_kv %s (1 .. 1024)"
                          % (head_dim, page_tokens, n_head_kv))
-    if pages.dim() != 2 or pages.shape[1] != width or pages.stride(1) != 1:
-        raise ValueError("pages has shape %s, not [n_pages, %d] with adjacent bytes" % (tuple(pages.shape), width))
-    _ints("table", table, device, None, None)
-    n_seq = table.shape[0]
-    _ints("lens", lens, device, n_seq)
+    shape, step = pages.shape, pages.stride()
+    if len(shape) != 2 or shape[1] != width or step[1] != 1:
+        raise ValueError("pages has shape %s, not [n_pages, %d] with adjacent bytes" % (tuple(shape), width))
+    tp = _ints(device, "table", table, 2)
+    n_seq, entries = table.shape
+    pitch = table.stride()[0]
+    if pitch < entries:
+        if n_seq > 1:
+            raise ValueError("the rows of table overlap")
+        pitch = entries
+    lp = _ints(device, "lens", lens, 1, n_seq)
     if cu is not None:
-        _ints("cu", cu, device, n_seq + 1)
-    elif n_seq != 1:
+        cp = _ints(device, "cu", cu, 1, n_seq + 1)
+    elif n_seq == 1:
+        cp = 0
+    else:
         raise ValueError("cu is needed for more than one sequence")
-    if n_seq > 1 and table.stride(0) < table.shape[1]:
-        raise ValueError("the rows of table overlap")
     if max_rows < 0:
         raise ValueError("max_rows is negative")
-    return _Cache(pages.data_ptr(), table.data_ptr(), lens.data_ptr(), cu.data_ptr() if cu is not None else None, pages.stride(0), pages.shape[0],
-                  max(table.stride(0), table.shape[1]), table.shape[1], n_seq, total, n_head_kv, head_dim, page_tokens, min(max_rows, total))
+    return CACHE.pack(pages.data_ptr(), tp, lp, cp, step[0], shape[0], pitch, entries, n_seq, total, n_head_kv, head_dim, page_tokens, min(max_rows, total))
 
 
 def kv4_page_bytes(n_head_kv, head_dim, page_tokens):
     """Bytes of a page of `page_tokens` tokens (32, 64, 128 or 256): 4.5 bits for each of K's and V's values, head_dim rounded up to 32."""
-    n = _library().ctamd_kv4_page_bytes(n_head_kv, head_dim, page_tokens)
+    if _lib is None:
+        load()
+    n = _lib.ctamd_kv4_page_bytes(n_head_kv, head_dim, page_tokens)
     if not n:
         raise ValueError("sizes not supported: head_dim is a multiple of 8 up to 256, page_tokens 32, 64, 128 or 256, n_head_kv 1 .. 1024")
     return n
@@ -173,25 +163,24 @@ def kv4_append(k, v, pages, table, lens, cu, max_rows, *, page_tokens):
 
     A group of 32 dims of a token becomes f16(d) * (code - 8), code 0 .. 15, d = the value of largest magnitude / -8 (the rounding of Q4_0 weights); values beyond
     +-65504 are stored as that.  A token whose K or V of a head holds a NaN makes every row that sees it NaN.  No two sequences of a call may write one page."""
-    if not isinstance(pages, torch.Tensor):
-        raise TypeError("pages is a uint8 tensor")
-    device = pages.device
-    kr, vr = _rows("k", k, device), _rows("v", v, device, k.shape)
-    c = _cache(pages, table, lens, cu, k.shape[0], k.shape[1], k.shape[2], page_tokens, max_rows)
-    with _On(device) as stream:
-        _call(_lib.ctamd_kv4_append(byref(c), byref(kr), byref(vr), stream))
+    device = _device_of("pages", pages)
+    kr = _rows(device, "k", k)
+    total, n_head_kv, head_dim = k.shape
+    vr = _rows(device, "v", v, k.shape)
+    c = _cache(device, pages, table, lens, cu, total, n_head_kv, head_dim, page_tokens, max_rows)
+    _launch(device, lambda stream: _lib.ctamd_kv4_append(c, kr, vr, stream))
 
 
 def kv4_read(pages, table, lens, cu, max_rows, total, *, n_head_kv, head_dim, page_tokens, dtype=torch.float16):
     """The last rows of every sequence as (k, v) [total, n_head_kv, head_dim]; 0 where there is no page or no position.  Rows of no sequence are undefined."""
     if dtype not in _TYPES:
         raise TypeError("dtype is float16, bfloat16 or float32")
-    c = _cache(pages, table, lens, cu, total, n_head_kv, head_dim, page_tokens, max_rows)
-    device = pages.device
-    with _On(device) as stream:
-        k = torch.empty((total, n_head_kv, head_dim), dtype=dtype, device=device)
-        v = torch.empty((total, n_head_kv, head_dim), dtype=dtype, device=device)
-        _call(_lib.ctamd_kv4_read(byref(c), byref(_rows("k", k, device)), byref(_rows("v", v, device)), stream))
+    device = _device_of("pages", pages)
+    c = _cache(device, pages, table, lens, cu, total, n_head_kv, head_dim, page_tokens, max_rows)
+    both = torch.empty((2, total, n_head_kv, head_dim), dtype=dtype, device=pages.device)
+    k, v = both.unbind(0)
+    kr, vr = _rows(device, "k", k), _rows(device, "v", v)
+    _launch(device, lambda stream: _lib.ctamd_kv4_read(c, kr, vr, stream))
     return k, v
 
 
@@ -200,71 +189,70 @@ def kv4_attention(q, pages, table, lens, cu, max_rows, *, n_head_kv, page_tokens
     reads KV head h // (n_head / n_head_kv), scores are q.k * scale (default 1 / sqrt(head_dim)).  A row that sees nothing becomes 0.  q is float16, bfloat16 or
     float32; the result has q's type, or is written into `out` [total, n_head, head_dim] of any of the three, where rows that belong to no sequence are left as they
     are.  Products are taken in float16 (K's codes and V's values; q scaled by a power of two per row, and p), everything else in float32."""
-    if not isinstance(pages, torch.Tensor):
-        raise TypeError("pages is a uint8 tensor")
-    device = pages.device
-    qr = _rows("q", q, device)
+    device = _device_of("pages", pages)
+    qr = _rows(device, "q", q)
     total, n_head, head_dim = q.shape
     if n_head_kv < 1 or n_head < 1 or n_head % n_head_kv:
         raise ValueError("%d query heads over %d KV heads" % (n_head, n_head_kv))
-    if qr.dim != 1 and head_dim > 1:
+    if q.stride()[2] != 1 and head_dim > 1:
         q = q.contiguous()
-        qr = _rows("q", q, device)
-    c = _cache(pages, table, lens, cu, total, n_head_kv, head_dim, page_tokens, max_rows)
-    with _On(device) as stream:
-        if out is None:
-            out = torch.empty((total, n_head, head_dim), dtype=q.dtype, device=device)
-        orow = _rows("out", out, device, q.shape)
-        n = _lib.ctamd_kv4_attention_ws(byref(c), n_head)
-        ws = torch.empty(n, dtype=torch.float32, device=device) if n else None
-        _call(_lib.ctamd_kv4_attention(byref(c), n_head, byref(qr), byref(orow), 1.0 / math.sqrt(head_dim) if scale is None else scale,
-                                       ws.data_ptr() if n else None, n, stream))
+        qr = _rows(device, "q", q)
+    c = _cache(device, pages, table, lens, cu, total, n_head_kv, head_dim, page_tokens, max_rows)
+    if out is None:
+        out = torch.empty((total, n_head, head_dim), dtype=q.dtype, device=q.device)
+    orow = _rows(device, "out", out, q.shape)
+    n = _lib.ctamd_kv4_attention_ws(c, n_head)
+    if n:
+        ws = torch.empty(n, dtype=torch.float32, device=q.device)
+        at = ws.data_ptr()
+    else:
+        at = None
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    _launch(device, lambda stream: _lib.ctamd_kv4_attention(c, n_head, qr, orow, scale, at, n, stream))
     return out
 
 
-def _tables(table, lens, refs, page_tokens, rows):
-    _library()
-    if not isinstance(table, torch.Tensor) or table.device.type != _device:
-        raise ValueError("table is a tensor in GPU memory")
-    device = table.device
-    _ints("table", table, device, None, None)
-    _ints("refs", refs, device, None)
-    if lens is not None:
-        _ints("lens", lens, device, table.shape[0])
+def _tables(device, table, lens, refs, page_tokens, rows=None):
+    """(the packed structure, outputs, what has to outlive the call)"""
+    tp = _ints(device, "table", table, 2)
+    n_seq, width = table.shape
+    rp = _ints(device, "refs", refs, 1)
+    lp = _ints(device, "lens", lens, 1, n_seq) if lens is not None else 0
     if page_tokens < 1:
         raise ValueError("page_tokens is positive")
-    if not table.is_contiguous():
+    if n_seq > 1 and table.stride()[0] != width:
         table = table.contiguous()
-    n = table.shape[0] if rows is None else rows
-    new = (torch.empty((n, table.shape[1]), dtype=torch.int32, device=device),
-           torch.empty((n,), dtype=torch.int32, device=device) if lens is not None else None, torch.empty_like(refs))
-    t = _Tables(table.data_ptr(), lens.data_ptr() if lens is not None else None, refs.data_ptr(), new[0].data_ptr(),
-                new[1].data_ptr() if lens is not None else None, new[2].data_ptr(), table.shape[0], table.shape[1], refs.shape[0], page_tokens)
-    return t, new, table
+        tp = table.data_ptr()
+    if rows is None:
+        rows = n_seq
+    on = refs.device
+    t = torch.empty((rows, width), dtype=_INT, device=on)
+    n = torch.empty((rows,), dtype=_INT, device=on) if lens is not None else None
+    r = torch.empty(refs.shape, dtype=_INT, device=on)
+    return TABLES.pack(tp, lp, rp, t.data_ptr(), n.data_ptr() if lens is not None else 0, r.data_ptr(), n_seq, width, refs.shape[0], page_tokens), (t, n, r), table
 
 
-def _pool(pages, refs):
-    if not isinstance(pages, torch.Tensor) or pages.device != refs.device:
+def _pool(device, pages, refs):
+    """(address, layers, bytes from layer to layer, bytes of a page)"""
+    if not isinstance(pages, torch.Tensor) or pages.get_device() != device:
         raise ValueError("pages is a tensor on the device of the tables")
-    if pages.dim() not in (2, 3) or pages.shape[-2] != refs.shape[0]:
-        raise ValueError("pages has shape %s: [n_pages, page] or [layers, n_pages, page] with %d pages" % (tuple(pages.shape), refs.shape[0]))
-    if pages.stride(-1) != 1 or pages.stride(-2) != pages.shape[-1]:
+    shape, step, e = pages.shape, pages.stride(), pages.element_size()
+    if len(shape) not in (2, 3) or shape[-2] != refs.shape[0]:
+        raise ValueError("pages has shape %s: [n_pages, page] or [layers, n_pages, page] with %d pages" % (tuple(shape), refs.shape[0]))
+    if step[-1] != 1 or step[-2] != shape[-1]:
         raise ValueError("the pages of a layer are not adjacent")
-    e = pages.element_size()
-    return (pages.data_ptr(), pages.shape[0], pages.stride(0) * e, pages.shape[-1] * e) if pages.dim() == 3 else (
-        pages.data_ptr(), 1, pages.shape[0] * pages.shape[1] * e, pages.shape[1] * e)
+    return (pages.data_ptr(), shape[0], step[0] * e, shape[2] * e) if len(shape) == 3 else (pages.data_ptr(), 1, shape[0] * shape[1] * e, shape[1] * e)
 
 
 def kv_fork(table, lens, refs, parents, *, page_tokens):
     """(table, lens, refs) of a batch whose sequence i continues sequence parents[i], sharing its pages: the batch may grow, shrink, permute and repeat, a parent
     outside [0, n_seq) makes an empty sequence (-1: freed).  A page whose last reference goes is free.  table [n_seq, width], refs [n_pages]."""
-    _library()
-    if not isinstance(parents, torch.Tensor) or parents.dim() != 1:
-        raise TypeError("parents is an int32 tensor with one dimension")
-    t, new, keep = _tables(table, lens, refs, page_tokens, parents.shape[0])
-    _ints("parents", parents, table.device, None)
-    with _On(table.device) as stream:
-        _call(_lib.ctamd_kv_fork(byref(t), parents.data_ptr(), parents.shape[0], stream))
+    device = _device_of("table", table)
+    at = _ints(device, "parents", parents, 1)
+    n_new = parents.shape[0]
+    t, new, keep = _tables(device, table, lens, refs, page_tokens, n_new)
+    _launch(device, lambda stream: _lib.ctamd_kv_fork(t, at, n_new, stream))
     return new
 
 
@@ -272,24 +260,25 @@ def kv_reserve(pages, table, lens, refs, add, *, page_tokens):
     """(table, lens, refs, short) with room for add[i] more tokens in sequence i: lens grows by it, pages are taken lowest free first in the order of the sequences,
     and a last page that others share is copied before its sequence writes it.  pages: [n_pages, ..] or [layers, n_pages, ..], any type.  short (int32, on the
     device): 0, or the pages that were missing, or -1 where a sequence outgrows its row of the table; then nothing has changed."""
-    t, new, keep = _tables(table, lens, refs, page_tokens, None)
-    device = table.device
-    _ints("add", add, device, table.shape[0])
-    p = _pool(pages, refs)
-    with _On(device) as stream:
-        short = torch.empty((), dtype=torch.int32, device=device)
-        ws = torch.empty(_lib.ctamd_kv_reserve_ws(table.shape[0], refs.shape[0]), dtype=torch.int32, device=device)
-        _call(_lib.ctamd_kv_reserve(byref(t), add.data_ptr(), p[0], p[1], p[2], p[3], short.data_ptr(), ws.data_ptr(), stream))
+    device = _device_of("table", table)
+    t, new, keep = _tables(device, table, lens, refs, page_tokens)
+    n_seq, n_pages = table.shape[0], refs.shape[0]
+    more = _ints(device, "add", add, 1, n_seq)
+    at, layers, layer_bytes, page_bytes = _pool(device, pages, refs)
+    short = torch.empty((), dtype=_INT, device=refs.device)
+    ws = torch.empty(_lib.ctamd_kv_reserve_ws(n_seq, n_pages), dtype=_INT, device=refs.device)
+    sp, wp = short.data_ptr(), ws.data_ptr()
+    _launch(device, lambda stream: _lib.ctamd_kv_reserve(t, more, at, layers, layer_bytes, page_bytes, sp, wp, stream))
     return new + (short,)
 
 
 def kv_compact(pages, table, refs):
     """(table, refs, used) after the pages in use have become pages 0 .. used - 1: those beyond move, in order, into the holes below.  used: int32, on the device."""
-    t, new, keep = _tables(table, None, refs, 1, None)
-    device = table.device
-    p = _pool(pages, refs)
-    with _On(device) as stream:
-        used = torch.empty((), dtype=torch.int32, device=device)
-        ws = torch.empty(_lib.ctamd_kv_compact_ws(refs.shape[0]), dtype=torch.int32, device=device)
-        _call(_lib.ctamd_kv_compact(byref(t), p[0], p[1], p[2], p[3], used.data_ptr(), ws.data_ptr(), stream))
+    device = _device_of("table", table)
+    t, new, keep = _tables(device, table, None, refs, 1)
+    at, layers, layer_bytes, page_bytes = _pool(device, pages, refs)
+    used = torch.empty((), dtype=_INT, device=refs.device)
+    ws = torch.empty(_lib.ctamd_kv_compact_ws(refs.shape[0]), dtype=_INT, device=refs.device)
+    up, wp = used.data_ptr(), ws.data_ptr()
+    _launch(device, lambda stream: _lib.ctamd_kv_compact(t, at, layers, layer_bytes, page_bytes, up, wp, stream))
     return new[0], new[2], used

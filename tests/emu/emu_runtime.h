@@ -63,6 +63,7 @@ static inline int __builtin_amdgcn_sdot4(int a, int b, int c, bool) {
     memcpy(y, &b, 4);
     return c + x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3];
 }
+static inline int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
 static inline int __ffsll(unsigned long long v) { return __builtin_ffsll((long long)v); }
 
 // ---- minimal hip host API shim (host memory stands in for device memory) --------------------------------------------

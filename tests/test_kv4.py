@@ -6,7 +6,6 @@ v with weights p, so an element is off by at most (2^-11 + 2^-11) A with A = sum
 factor within exp(+-e): 2 e A.  A score's error: f32 sums, (D + 8) 2^-24 scale sum |q| |k|; the exponent's argument, (4 |s| + 8) 2^-23; queries that are not
 halves already, 2^-11 scale sum |q| |k| (float32) or the part below f16's range after the row's power of two, 2^-25 max |q| scale sum |k| (bf16); and in the
 many-row kernel K's values as halves, 2^-11 scale sum |q| |k|.  The result's own rounding is half a step of its type."""
-import ctypes
 import math
 import os
 import re
@@ -34,7 +33,7 @@ def dev(request):
         ops.load(HIP_LIB)
         yield torch.device("cuda:0")
     ops._lib = None
-    ops._device = "cuda"
+    ops._on_gpu = True
 
 
 # ---- the format, from its definition ------------------------------------------------------------------------------------------------------------
@@ -621,7 +620,7 @@ def test_refusals(dev):
         with pytest.raises(ValueError):
             call(**bad)
     for call, bad in [(att, dict(q=q.double())), (att, dict(q=q.int())), (att, dict(table=table.long())), (att, dict(lens=n.float())), (att, dict(pages=p.short())),
-                      (att, dict(out=q.double())), (app, dict(k=k.int())), (app, dict(pages=None))]:
+                      (att, dict(out=q.double())), (app, dict(k=k.int())), (app, dict(pages=None)), (app, dict(table=None))]:
         with pytest.raises(TypeError):
             call(**bad)
     shifted = torch.zeros(p.numel() + 16, dtype=torch.uint8, device=dev)[8:8 + p.numel()].view(p.shape)
@@ -669,11 +668,11 @@ def test_c_interface(hip_lib):
     lib = ops.load(hip_lib)
     try:
         assert lib.ctamd_kv4_append(None, None, None, None) == -1 and b"null cache" in lib.ctamd_ops_error()
-        c = ops._Cache(None, None, None, None, 36864, 0, 1, 1, 1, 1, 2, 64, 32, 1)
-        assert lib.ctamd_kv4_append(ctypes.byref(c), None, None, None) == -1 and b"null rows" in lib.ctamd_ops_error()
+        c = ops.CACHE.pack(0, 0, 0, 0, 36864, 0, 1, 1, 1, 1, 2, 64, 32, 1)
+        assert lib.ctamd_kv4_append(c, None, None, None) == -1 and b"null rows" in lib.ctamd_ops_error()
         assert lib.ctamd_kv_fork(None, None, 0, None) == -1 and lib.ctamd_kv_reserve(None, None, None, 0, 0, 0, None, None, None) == -1
-        t = ops._Tables(4096, 8192, 12288, 4096, 16384, 20480, 1, 2, 3, 4)
-        assert lib.ctamd_kv_fork(ctypes.byref(t), 24576, 1, None) == -1 and b"overlaps an input" in lib.ctamd_ops_error()
-        assert lib.ctamd_kv_compact(ctypes.byref(ops._Tables(4096, None, 12288, 32768, None, 20480, 1, 2, 3, 1)), 16, 1, 48, 16, None, None, None) == -1
+        t = ops.TABLES.pack(4096, 8192, 12288, 4096, 16384, 20480, 1, 2, 3, 4)
+        assert lib.ctamd_kv_fork(t, 24576, 1, None) == -1 and b"overlaps an input" in lib.ctamd_ops_error()
+        assert lib.ctamd_kv_compact(ops.TABLES.pack(4096, 0, 12288, 32768, 0, 20480, 1, 2, 3, 1), 16, 1, 48, 16, None, None, None) == -1
     finally:
         ops._lib = None
