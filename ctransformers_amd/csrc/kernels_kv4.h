@@ -140,13 +140,15 @@ DEV void kv4_load8(float (&x)[8], const Kv4Rows& r, long long at) {
 // A query row's pieces as halves: N pieces of eight dims, piece k at at + 8 * (k * step + lane's), dims from head_dim on are zeros.  Rows that f16 may not hold (bf16,
 // f32) are scaled by a power of two that brings the row's largest value into [1, 2) — all lanes that hold pieces of a row agree on it through `across` — so that bf16
 // stays exact but for values below 2^-17 of the largest.  Returns the inverse of the scale.
-template <int N, class Across> DEV float kv4_query(u32x4 (&q)[N], const Kv4Rows& r, long long at, int d0, int step, int head_dim, bool on, Across across) {
+// A negative `scale` goes into the query's sign: scores can then be compared before they are scaled.
+template <int N, class Across> DEV float kv4_query(u32x4 (&q)[N], const Kv4Rows& r, long long at, int d0, int step, int head_dim, bool on, float scale, Across across) {
+    const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;
     if (r.type == KV4_F16) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const bool in = on && d0 + step * k < head_dim;
             q[k] = kv4_load8_raw(r, in ? at + d0 + step * k : at);
-            if (!in) q[k] = u32x4_of(0, 0, 0, 0);
+            q[k] = in ? u32x4_of(q[k][0] ^ flip, q[k][1] ^ flip, q[k][2] ^ flip, q[k][3] ^ flip) : u32x4_of(0, 0, 0, 0);
         }
         return 1.0f;
     }
@@ -164,9 +166,12 @@ template <int N, class Across> DEV float kv4_query(u32x4 (&q)[N], const Kv4Rows&
     if (e > 0 && e < 254) { up = float_of((uint32_t)(254 - e) << 23); down = float_of((uint32_t)e << 23); }
 #pragma unroll
     for (int k = 0; k < N; ++k)
-        q[k] = u32x4_of(kv4_cvt2(x[k][0] * up, x[k][1] * up), kv4_cvt2(x[k][2] * up, x[k][3] * up), kv4_cvt2(x[k][4] * up, x[k][5] * up), kv4_cvt2(x[k][6] * up, x[k][7] * up));
+        q[k] = u32x4_of(kv4_cvt2(x[k][0] * up, x[k][1] * up) ^ flip, kv4_cvt2(x[k][2] * up, x[k][3] * up) ^ flip, kv4_cvt2(x[k][4] * up, x[k][5] * up) ^ flip,
+                        kv4_cvt2(x[k][6] * up, x[k][7] * up) ^ flip);
     return down;
 }
+// the factor of a score in front of exp2: positive, also for a scale of 0 (whose scores are then as good as equal), so that -inf stays what it is
+DEV float kv4_factor(float scale, float down, float unit) { return fmaxf(fabsf(scale) * 1.44269504088896f * down * unit, 1e-30f); }
 // eight neighbouring dims out; vec: as for loads
 DEV void kv4_store8(void* p, long long at, int type, int vec, const float (&x)[8]) {
     if (vec && type != KV4_F32) {
@@ -394,10 +399,11 @@ DEV Kv4Range kv4_range(const Kv4Attn& a, int b, int tile, int tile_rows, int par
 
 // kv4_decode_kernel: the work of all units — a unit is a (sequence, KV head, row tile) — stands in one line, which is cut into equal shares, one per workgroup, as
 // many as are resident at once.  So every workgroup has the same work whatever the sequences' lengths are.  A unit's work is its blocks and, before them, kUnitCost
-// blocks' worth for beginning and ending it (~6 us: the queries, the first loads, the waves' results joined; four waves stream a block each in about that time).
+// blocks' worth for beginning and ending it: the queries, the first loads, the waves' results joined, one latency after the other.  (64 sequences of 0 .. 8192 tokens,
+// 8 KV heads: 98 us at 4 blocks, 75 at 10, 70.5 at 14, 71 at 20, 72 at 28, 75 at 40.)
 // Only the first and the last unit of a share can be a part of one; a part that does not begin its unit goes to the share's first place in the workspace, one that
 // begins it to the second, whole units go straight out.  The line follows from lens and cu, which only the device knows: every wave sums it up for itself.
-constexpr int kUnitCost = 4;
+constexpr int kUnitCost = 16;
 struct Kv4Line { int before, all, per; };                     // (the host refuses tables with room for 2^31 blocks)
 DEV int kv4_unit_blocks(const Kv4Attn& a, int nq, int len) {   // blocks of each of a sequence's units (one, all masked, where there is nothing to see), 0: no rows
     if (nq <= 0) return 0;
@@ -556,11 +562,11 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
         const int tok = on ? r / a.rep : 0;
         lim[n] = on ? len - nq + tok + 1 : 0;
         const long long at = (long long)(lo + tok) * a.q.row + (long long)(kvh * a.rep + (on ? r - tok * a.rep : 0)) * a.q.head;
-        const float down = kv4_query<G>(q[n], a.q, at, 8 * i, 32, c.head_dim, on, [](float v) { v = fmaxf(v, lane_xor16(v)); return fmaxf(v, lane_xor32(v)); });
+        const float down = kv4_query<G>(q[n], a.q, at, 8 * i, 32, c.head_dim, on, a.scale, [](float v) { v = fmaxf(v, lane_xor16(v)); return fmaxf(v, lane_xor32(v)); });
 #pragma unroll
         for (int g = 0; g < G; ++g)   // -8 sum(Q) of the group in every row of the product: A all -8 (f16 bits 0x8008: -8 * 2^-24, as the codes are)
             cq[n][g] = mfma_f16_16x16x32(u32x4_of(0x80088008u, 0x80088008u, 0x80088008u, 0x80088008u), q[n][g], f32x4_splat(0.0f));
-        sc2[n] = a.scale * 1.44269504088896f * 16777216.0f * down;
+        sc2[n] = kv4_factor(a.scale, down, 16777216.0f);
         mx[n] = -INFINITY;
         sum[n] = 0.0f;
 #pragma unroll
@@ -611,19 +617,20 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
         }
         kv4_fetch_k<G>(kc, ks, nxt, m, i);
         {
-            const bool edge = p0 + 32 > free_lim || p0 + 32 > there;
             u32x4 P[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float top = -INFINITY;
+                if (p0 + 32 > free_lim || p0 + 32 > there) {
+                    const int left = here ? lim[n] - p0 - 4 * i : -1;   // tokens of this lane's from here on that the row does not see
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                    for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[n][t][e] *= sc2[n];
-                        if (edge && (p0 + 16 * t + 4 * i + e >= lim[n] || !here)) s[n][t][e] = -INFINITY;
-                        top = fmaxf(top, s[n][t][e]);
-                    }
+                        for (int e = 0; e < 4; ++e) s[n][t][e] = 16 * t + e >= left ? -INFINITY : s[n][t][e];
+                }
+                float top = s[n][0][0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) top = fmaxf(top, s[n][e / 4][e & 3]);
+                top *= sc2[n];
                 if (__ballot(top > mx[n] + 8.0f)) {   // (also the first block: -inf + 8)
                     top = fmaxf(top, lane_xor16(top));
                     top = fmaxf(top, lane_xor32(top));
@@ -636,13 +643,13 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
 #pragma unroll
                         for (int e = 0; e < 4; ++e) O[n][j][e] *= f;
                 }
-                const float base = mx[n] == -INFINITY ? 0.0f : mx[n];
+                const float base = mx[n] == -INFINITY ? 0.0f : -mx[n];
                 uint32_t pk[4];
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; e += 2) {
-                        const float x = exp2_fast(s[n][t][e] - base), y = exp2_fast(s[n][t][e + 1] - base);
+                        const float x = exp2_fast(fmaf(s[n][t][e], sc2[n], base)), y = exp2_fast(fmaf(s[n][t][e + 1], sc2[n], base));
                         sum[n] += x;
                         sum[n] += y;
                         pk[2 * t + e / 2] = kv4_cvt2(x, y);   // the probabilities as halves: 2^-12 of each, independent of one another
@@ -821,7 +828,7 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
     CT_DYN_SMEM(smem);
     __shared__ int here[4];   // [buffer][block]: the block is there
     const Kv4Cache& c = a.c;
-    const int tid = (int)threadIdx.x, lane = lane_id(), w = wave_id(), n = lane & 31, h = lane >> 5;
+    const int lane = lane_id(), w = uniform_int(wave_id()), tid = 64 * w + lane, n = lane & 31, h = lane >> 5;
     // workgroup -> (pair, split, tile): ids that are equal modulo 8 share an XCD
     const int pairs = c.n_seq * c.n_head_kv, per_pair = a.tiles * a.nsplit, id = (int)blockIdx.x;
     const int pair = (id & 7) + 8 * ((id >> 3) / per_pair), slot = (id >> 3) % per_pair;
@@ -836,9 +843,9 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
     const int tok = on ? r / a.rep : 0, head = kvh * a.rep + (on ? r % a.rep : 0);
     const int lim = on ? rg.len - rg.nq + tok + 1 : 0;
     u32x4 q[2 * G];
-    const float down = kv4_query<2 * G>(q, a.q, (long long)(rg.lo + tok) * a.q.row + (long long)head * a.q.head, 8 * h, 16, c.head_dim, on,
+    const float down = kv4_query<2 * G>(q, a.q, (long long)(rg.lo + tok) * a.q.row + (long long)head * a.q.head, 8 * h, 16, c.head_dim, on, a.scale,
                                         [](float v) { return fmaxf(v, lane_xor32(v)); });
-    const float sc2 = a.scale * 1.44269504088896f * down;
+    const float sc2 = kv4_factor(a.scale, down, 1.0f);
     float mx = -INFINITY, sum = 0.0f;
     f32x16 O[G];
 #pragma unroll
@@ -851,15 +858,15 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
     const int wfree = 32 * w < rg.n_rows ? rg.len - rg.nq + (tile * 128 + 32 * w) / a.rep + 1 : 0;
 
     // staging: a thread unpacks, of one block of the pair, K's G dwords of (token st, quad si) and V's dims sd, sd + 32, .. of the tokens' eight si
-    const int sb = tid >> 7, st = (tid >> 2) & 31, si = tid & 3, sd = tid & 31, ve = (tid >> 5) & 3;
+    const int sb = w >> 1, st = (tid >> 2) & 31, si = tid & 3, sd = tid & 31, ve = (tid >> 5) & 3;   // (sb: the same for a whole wave)
     uint32_t kc[G], ks[G], vc[G], vs[G][4];
     bool got = false;
     int pid = -1;
-    auto look_up = [&](int blk) { pid = blk + sb < end ? kv4_page_of(c, b, uniform_int(blk + sb)) : -1; };   // (sb is the same for a whole wave)
-    auto fetch = [&](int blk) {
+    auto look_up = [&](int blk) { pid = blk + sb < end ? kv4_page_of(c, b, blk + sb) : -1; };
+    auto fetch = [&](int blk) {   // where there is no block the pool's first is read, and masked
         const uint8_t* p = kv4_in_page(c, pid, kvh, blk + sb);
         got = p != nullptr;
-        if (!got) return;
+        p = got ? p : c.pages;
         kv4_ldw<G>(kc, p + ((st * 4 + si) * G) * 4);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -874,21 +881,22 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
         unsigned char* kb = smem + (buf * 2 + sb) * L::BLK;
         unsigned char* vb = kb + L::KB;
         const int p0 = (blk + sb) * 32;
-        uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-        if (p0 + 32 > rg.len) {
+        const int there = got ? rg.len : 0;
+        if (p0 + 32 > there) {   // V past the sequence's end (K's scores are masked there)
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
                 const int t0 = p0 + 16 * (p / 2) + 4 * ve + 2 * (p & 1);
-                keep[p] = (t0 < rg.len ? 0xFFFFu : 0u) | (t0 + 1 < rg.len ? 0xFFFF0000u : 0u);
+                const uint32_t keep = (t0 < there ? 0xFFFFu : 0u) | (t0 + 1 < there ? 0xFFFF0000u : 0u);
+#pragma unroll
+                for (int g = 0; g < G; ++g) vs[g][p] &= keep;
             }
         }
         if ((tid & 127) == 0) here[buf * 2 + sb] = got;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const uint32_t s = got ? ks[g] | (ks[g] << 16) : 0u;
-            lds_st16(kb + (4 * g + si) * L::KC + st * 16, got ? kv4_values(kc[g], s, s, s, s) : u32x4_of(0, 0, 0, 0));
-            lds_st16(vb + (ve * 32 * G + 32 * g + sd) * 16,
-                     got ? kv4_values(vc[g], vs[g][0] & keep[0], vs[g][1] & keep[1], vs[g][2] & keep[2], vs[g][3] & keep[3]) : u32x4_of(0, 0, 0, 0));
+            const uint32_t s = ks[g] | (ks[g] << 16);
+            lds_st16(kb + (4 * g + si) * L::KC + st * 16, kv4_values(kc[g], s, s, s, s));
+            lds_st16(vb + (ve * 32 * G + 32 * g + sd) * 16, kv4_values(vc[g], vs[g][0], vs[g][1], vs[g][2], vs[g][3]));
         }
     };
     const int tk = 16 * ((n >> 3) & 1) + 8 * (n >> 4) + 4 * ((n >> 2) & 1) + (n & 3);   // the token that this lane's row of K's operand is
@@ -903,20 +911,19 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
                 const u32x4 kf = lds_ld16(smem + (buf * 2 + k) * L::BLK + (2 * g + h) * L::KC + tk * 16);
                 S[k] = g == 0 ? mfma_f16_32x32x16(kf, q[g]) : mfma_f16_32x32x16_acc(kf, q[g], S[k]);
             }
-        const bool gone0 = !here[buf * 2], gone1 = !here[buf * 2 + 1];
-        const bool edge = p0 + 64 > wfree || gone0 || gone1;
-        float top = -INFINITY;
+        const int here0 = uniform_int(here[buf * 2]), here1 = uniform_int(here[buf * 2 + 1]);
+        if (p0 + 64 > wfree || !here0 || !here1) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+            for (int k = 0; k < 2; ++k) {
+                const int left = (k ? here1 : here0) ? lim - p0 - 32 * k - 4 * h : -1;   // tokens of this lane's from here on that the row does not see
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                S[k][e] *= sc2;
-                if (edge) {
-                    const int p = p0 + 32 * k + 16 * ((e >> 2) & 1) + 8 * (e >> 3) + 4 * h + (e & 3);
-                    if (p >= lim || (k ? gone1 : gone0)) S[k][e] = -INFINITY;
-                }
-                top = fmaxf(top, S[k][e]);
+                for (int e = 0; e < 16; ++e) S[k][e] = 16 * ((e >> 2) & 1) + 8 * (e >> 3) + (e & 3) >= left ? -INFINITY : S[k][e];
             }
+        }
+        float top = S[0][0];
+#pragma unroll
+        for (int e = 1; e < 32; ++e) top = fmaxf(top, S[e / 16][e & 15]);
+        top *= sc2;
         if (__ballot(top > mx + 8.0f)) {
             top = fmaxf(top, lane_xor32(top));
             const float now = fmaxf(mx, top);
@@ -928,7 +935,7 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
 #pragma unroll
                 for (int e = 0; e < 16; ++e) O[g][e] *= f;
         }
-        const float base = mx == -INFINITY ? 0.0f : mx;
+        const float base = mx == -INFINITY ? 0.0f : -mx;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const unsigned char* vb = smem + (buf * 2 + k) * L::BLK + L::KB;
@@ -937,7 +944,7 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
                 uint32_t pk[4];
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    const float x = exp2_fast(S[k][8 * t + e] - base), y = exp2_fast(S[k][8 * t + e + 1] - base);
+                    const float x = exp2_fast(fmaf(S[k][8 * t + e], sc2, base)), y = exp2_fast(fmaf(S[k][8 * t + e + 1], sc2, base));
                     sum += x;
                     sum += y;
                     pk[e / 2] = kv4_cvt2(x, y);
@@ -948,7 +955,7 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
             }
         }
     };
-    if (begin < end) {
+    if (begin < end && c.n_pages > 0) {
         look_up(begin);
         fetch(begin);
         look_up(begin + 2);
