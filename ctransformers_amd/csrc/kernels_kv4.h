@@ -64,6 +64,13 @@ static inline uint32_t kv4_op2(uint32_t a, uint32_t b, bool mul) {
 static inline uint32_t kv4_add2(uint32_t a, uint32_t b) { return kv4_op2(a, b, false); }
 static inline uint32_t kv4_mul2(uint32_t a, uint32_t b) { return kv4_op2(a, b, true); }
 static inline uint32_t kv4_cvt2(float a, float b) { return (uint32_t)f32_to_f16_bits(a) | ((uint32_t)f32_to_f16_bits(b) << 16); }
+static inline uint32_t kv4_fma2(uint32_t a, uint32_t b, uint32_t c) {   // (used where the result is exact)
+    uint32_t r = 0;
+    for (int s = 0; s < 32; s += 16) r |= (uint32_t)f32_to_f16_bits(fmaf(f16_bits_to_f32((uint16_t)(a >> s)), f16_bits_to_f32((uint16_t)(b >> s)), f16_bits_to_f32((uint16_t)(c >> s)))) << s;
+    return r;
+}
+static inline float kv4_sum2(uint32_t a, float c) { return c + (f16_bits_to_f32((uint16_t)(a & 0xFFFFu)) + f16_bits_to_f32((uint16_t)(a >> 16))); }
+static inline uint32_t kv4_and_or(uint32_t a, uint32_t b, uint32_t c) { return (a & b) | c; }
 static inline float exp2_fast(float x) { return exp2f(x); }
 static inline u32x4 u32x4_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return u32x4{{a, b, c, d}}; }
 static inline f32x4 f32x4_splat(float x) { return f32x4{{x, x, x, x}}; }
@@ -75,6 +82,15 @@ typedef _Float16 kv4_h2 __attribute__((ext_vector_type(2)));
 DEV uint32_t kv4_add2(uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(kv4_h2, a) + __builtin_bit_cast(kv4_h2, b)); }
 DEV uint32_t kv4_mul2(uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(kv4_h2, a) * __builtin_bit_cast(kv4_h2, b)); }
 DEV uint32_t kv4_cvt2(float a, float b) { return __builtin_bit_cast(uint32_t, kv4_h2{(_Float16)a, (_Float16)b}); }   // nearest even
+DEV uint32_t kv4_fma2(uint32_t a, uint32_t b, uint32_t c) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(kv4_h2, a), __builtin_bit_cast(kv4_h2, b), __builtin_bit_cast(kv4_h2, c)));
+}
+DEV float kv4_sum2(uint32_t a, float c) { return __builtin_amdgcn_fdot2(__builtin_bit_cast(kv4_h2, a), kv4_h2{(_Float16)1.0f, (_Float16)1.0f}, c, false); }
+DEV uint32_t kv4_and_or(uint32_t a, uint32_t b, uint32_t c) {   // one instruction; the compiler makes two
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "s"(b), "v"(c));   // (one scalar operand an instruction)
+    return r;
+}
 DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32: 1 ulp, results below 2^-126 are 0
 DEV u32x4 u32x4_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return u32x4{a, b, c, d}; }
 DEV f32x4 f32x4_splat(float x) { return f32x4{x, x, x, x}; }
@@ -462,9 +478,11 @@ DEV int kv4_find(const Kv4Attn& a, int tile_rows, int x, int& begin) {
 // Eight halves of the dword's codes minus 8, times the scales of their tokens (or one scale for all): f16 products, one rounding (2^-11 of a value whose step is
 // 1/8 of the group's largest) — the matrix instruction takes halves.
 DEV u32x4 kv4_values(uint32_t w, uint32_t s0, uint32_t s1, uint32_t s2, uint32_t s3) {
-    const uint32_t M = 0x000F000Fu, K = 0x64006400u, B = 0xE408E408u;   // 1024 + code, exactly; -1032
-    return u32x4_of(kv4_mul2(kv4_add2((w & M) | K, B), s0), kv4_mul2(kv4_add2(((w >> 4) & M) | K, B), s1),
-                    kv4_mul2(kv4_add2(((w >> 8) & M) | K, B), s2), kv4_mul2(kv4_add2(((w >> 12) & M) | K, B), s3));
+    // halves 1024 + code (low nibbles of the bytes) and 1024 + 16 code (high nibbles: no shift); - 1032 and / 16 - 72 give code - 8, all of it exact
+    const uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u, K = 0x64006400u, u = w >> 8;
+    const uint32_t v0 = kv4_add2(kv4_and_or(w, lo, K), 0xE408E408u), v1 = kv4_fma2(kv4_and_or(w, hi, K), 0x2C002C00u, 0xD480D480u);
+    const uint32_t v2 = kv4_add2(kv4_and_or(u, lo, K), 0xE408E408u), v3 = kv4_fma2(kv4_and_or(u, hi, K), 0x2C002C00u, 0xD480D480u);
+    return u32x4_of(kv4_mul2(v0, s0), kv4_mul2(v1, s1), kv4_mul2(v2, s2), kv4_mul2(v3, s3));
 }
 
 // Few rows (a token step, a handful of drafted tokens): a wave takes whole blocks.  16x16x32 matrix products, transposed so that a query row is a COLUMN of both:
@@ -650,9 +668,8 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
 #pragma unroll
                     for (int e = 0; e < 4; e += 2) {
                         const float x = exp2_fast(fmaf(s[n][t][e], sc2[n], base)), y = exp2_fast(fmaf(s[n][t][e + 1], sc2[n], base));
-                        sum[n] += x;
-                        sum[n] += y;
-                        pk[2 * t + e / 2] = kv4_cvt2(x, y);   // the probabilities as halves: 2^-12 of each, independent of one another
+                        pk[2 * t + e / 2] = kv4_cvt2(x, y);   // the probabilities as halves: 2^-11 of each at most, independent of one another; their sum is of the halves
+                        sum[n] = kv4_sum2(pk[2 * t + e / 2], sum[n]);
                     }
                 P[n] = u32x4_of(pk[0], pk[1], pk[2], pk[3]);
             }
@@ -831,10 +848,19 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
     const int lane = lane_id(), w = uniform_int(wave_id()), tid = 64 * w + lane, n = lane & 31, h = lane >> 5;
     // workgroup -> (pair, split, tile): ids that are equal modulo 8 share an XCD
     const int pairs = c.n_seq * c.n_head_kv, per_pair = a.tiles * a.nsplit, id = (int)blockIdx.x;
-    const int pair = (id & 7) + 8 * ((id >> 3) / per_pair), slot = (id >> 3) % per_pair;
-    if (pair >= pairs) return;
+    const int j = id >> 3, np = (pairs - (id & 7) + 7) >> 3;   // pairs of this XCD
+    if (np <= 0 || j >= np * per_pair) return;
+    int pair, slot;
+    if ((int)gridDim.x <= a.want_parts) {   // all resident, two a CU: the tiles that see most first, then those that see least upwards, so that a CU has one of each
+        pair = (id & 7) + 8 * (j % np);
+        slot = j / np;
+        if (slot >= (per_pair + 1) / 2) slot = per_pair - 1 - (slot - (per_pair + 1) / 2);
+    } else {                                // one pair after the other, its long tiles first
+        pair = (id & 7) + 8 * (j / per_pair);
+        slot = j % per_pair;
+    }
     const int split = slot % a.nsplit, tile = a.tiles - 1 - slot / a.nsplit;
-    const int b = pair / c.n_head_kv, kvh = pair % c.n_head_kv;
+    const int b = uniform_int(pair / c.n_head_kv), kvh = pair - b * c.n_head_kv;
     const Kv4Range rg = kv4_range(a, b, tile, 128, kv4_part(a));
     if (rg.n_rows <= 0 || (split >= rg.parts && split > 0)) return;
 
@@ -945,9 +971,8 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
                     const float x = exp2_fast(fmaf(S[k][8 * t + e], sc2, base)), y = exp2_fast(fmaf(S[k][8 * t + e + 1], sc2, base));
-                    sum += x;
-                    sum += y;
                     pk[e / 2] = kv4_cvt2(x, y);
+                    sum = kv4_sum2(pk[e / 2], sum);
                 }
                 const u32x4 P = u32x4_of(pk[0], pk[1], pk[2], pk[3]);
 #pragma unroll
