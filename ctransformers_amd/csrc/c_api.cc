@@ -233,6 +233,24 @@ long long ctamd_resident_replays(ctransformers_llm* llm) {   // requests evaluat
     for (int s = 0; s < llm->pipe.n_stages(); ++s) n += llm->pipe.stage(s).resident_replays();
     return n;
 }
+// contexts of a handle with the 4-bit paged cache (single-GPU handles: one stage)
+static int context_result(bool ok, const std::string& err) {
+    if (!ok) fprintf(stderr, "ctransformers_amd: %s\n", err.c_str());
+    return ok ? 0 : -1;
+}
+int ctamd_n_contexts(ctransformers_llm* llm) { return llm->engine().n_contexts(); }
+int ctamd_context_length(ctransformers_llm* llm, int context) { return llm->engine().context_length_of(context); }
+int ctamd_context_use(ctransformers_llm* llm, int context) { std::string err; const bool ok = llm->engine().context_use(context, err); return context_result(ok, err); }
+int ctamd_context_fork(ctransformers_llm* llm, int src, int dst) { std::string err; const bool ok = llm->engine().context_fork(src, dst, err); return context_result(ok, err); }
+int ctamd_context_free(ctransformers_llm* llm, int context) { std::string err; const bool ok = llm->engine().context_free(context, err); return context_result(ok, err); }
+int ctamd_context_compact(ctransformers_llm* llm) {
+    std::string err;
+    const int used = llm->engine().context_compact(err);
+    if (used < 0) fprintf(stderr, "ctransformers_amd: %s\n", err.c_str());
+    return used;
+}
+long long ctamd_kv4_launches(ctransformers_llm* llm) { return llm->engine().kv4_launches(); }
+int ctamd_debug_read_q(ctransformers_llm* llm, unsigned short* dst, int n_tok) { return llm->engine().debug_read_q(dst, n_tok); }
 int ctamd_falcon_fold(ctransformers_llm* llm) { return llm->engine().falcon_fold() ? 1 : 0; }
 int ctamd_debug_read_attn_out(ctransformers_llm* llm, float* dst, int n_tok) { return llm->engine().debug_read_attn_out(dst, n_tok); }
 int ctamd_debug_read_kv(ctransformers_llm* llm, int layer, unsigned short* k, unsigned short* v) { return llm->engine().debug_read_kv(layer, k, v); }

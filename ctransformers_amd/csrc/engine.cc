@@ -20,6 +20,7 @@
 #include "kernels_pg.h"
 #include "kernels_raw32.h"
 #include "kernels_mm8.h"
+#include "kv4.h"
 
 namespace ctamd {
 
@@ -65,6 +66,8 @@ void Engine::free_all() {
     dev_allocs_.clear();
     if (h_logits_) (void)hipHostFree(h_logits_);   // h_emb_ lives in the same pinned block
     if (h_scalars_) (void)hipHostFree(h_scalars_);
+    if (h_kv_) (void)hipHostFree(h_kv_);
+    h_kv_ = nullptr;
     h_logits_ = h_emb_ = nullptr;
     h_scalars_ = nullptr;
 #ifndef CT_EMU
@@ -555,7 +558,10 @@ void Engine::fill_attn_args(AttnArgsX& ax, uint16_t* kc, uint16_t* vc, int nt) {
     if (trace_site_ && (!strcmp(trace_site_, "attn") || !strcmp(trace_site_, "qa"))) ax.trace = trace_buf_;
 }
 
+#include "engine_kv4.h"
+
 void Engine::launch_attention(uint16_t* kc, uint16_t* vc, int nt) {
+    if (kv4_) { kv4_attend(kc, vc, nt); return; }
     const int hd = hp_.head_dim();
     AttnArgsX ax = AttnArgsX();
     fill_attn_args(ax, kc, vc, nt);
@@ -1220,6 +1226,7 @@ bool Engine::req_begin(const int* tokens, int n, int n_past, int batch, std::str
         if (tk < 0 || tk >= hp_.n_vocab) { err = "token id out of range"; return false; }
         h_scalars_[4 + i] = tk;
     }
+    if (kv4_ && !kv4_room(n_past, n, err)) return false;
     h_scalars_[0] = 0;           // step
     h_scalars_[1] = n_past;      // position of the first token of this request
     h_scalars_[2] = n_past + n;  // end of the eval; with [3] the attention kernels derive the reference batch each token belongs to
@@ -1313,6 +1320,7 @@ bool Engine::req_wait(int n, int n_past, std::string& err) {
               "its own grid (is the device shared?): the request is evaluated again with the forms that need no residency";
         return false;
     }
+    if (!kv4_err_.empty()) { err = kv4_err_; kv4_err_.clear(); return false; }
     have_logits_ = l1_ == hp_.n_layer;
     last_token_ = h_scalars_[4 + n - 1];
     last_pos_ = n_past + n - 1;
@@ -1388,13 +1396,23 @@ int Engine::read_stamps(unsigned long long* out, int max) {
 }
 
 int Engine::debug_read_kv(int layer, uint16_t* k, uint16_t* v) {
-    if (layer < l0_ || layer >= l1_ || !kcache_ || !vcache_) return -1;
+    if (kv4_ || layer < l0_ || layer >= l1_ || !kcache_ || !vcache_) return -1;
     (void)hipSetDevice(device_);
     (void)hipStreamSynchronize(stream_);
     const int G = hp_.n_embd_gqa();
     (void)hipMemcpy(k, kcache_ + (size_t)(layer - l0_) * n_ctx_ * G, (size_t)n_ctx_ * G * 2, hipMemcpyDeviceToHost);
     (void)hipMemcpy(v, vcache_ + (size_t)(layer - l0_) * v_stride_ * G, (size_t)v_stride_ * G * 2, hipMemcpyDeviceToHost);
     return v_stride_;
+}
+
+// Test hook: the fp16 query rows (rotated) of the last layer, of the last chunk (n_tok rows) or, n_tok = 0, the last token step.
+int Engine::debug_read_q(uint16_t* dst, int n_tok) {
+    const uint16_t* q = n_tok ? q_f16_b_ : q_f16_;
+    if (!q || n_tok < 0 || n_tok > pf_cap_) return -1;
+    (void)hipSetDevice(device_);
+    (void)hipStreamSynchronize(stream_);
+    (void)hipMemcpy(dst, q, (size_t)std::max(1, n_tok) * hp_.n_embd * 2, hipMemcpyDeviceToHost);
+    return hp_.n_embd;
 }
 
 // Test hook: the attention output rows of the last chunk launched (last layer of this stage), n_tok x n_embd floats.
@@ -1419,6 +1437,7 @@ bool Engine::decode_burst(int n, double* us_per_token, std::string& err) {
     if (last_pos_ + 1 + n >= n_ctx_ || n < 1 || n > 100) { err = "decode_burst: would run past the context"; return false; }
     if (!drain_spec(err)) return false;
     if (!ensure_graphs(err)) return false;
+    if (kv4_ && !kv4_room(last_pos_ + 1, n, err)) return false;
     // the cursor as the next eval would set it; the token ids are whatever the last request left in d_tokens_ (timing only) — with
     // continuation graphs the burst IS the greedy chain (each head launch hands the next step its token)
     h_scalars_[0] = 0; h_scalars_[1] = last_pos_ + 1; h_scalars_[2] = last_pos_ + 1 + (graph_cont_[0] ? 1 : n); h_scalars_[3] = 0;

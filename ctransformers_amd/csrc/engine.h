@@ -15,6 +15,7 @@
 
 struct MatvecArgs;
 struct AttnArgsX;
+struct Kv4Cache;
 
 namespace ctamd {
 
@@ -132,6 +133,15 @@ class Engine {
     bool resident_timeout();
     void disable_resident_forms();
     long long resident_replays() const { return resident_replays_; }
+    // contexts of a handle with the 4-bit paged cache (engine_kv4.h); 1 without it
+    int n_contexts() const { return kv4_ ? (int)ctxs_.size() : 1; }
+    int context_length_of(int i) const { return kv4_ && i >= 0 && i < (int)ctxs_.size() ? ctxs_[i].len : -1; }
+    bool context_use(int i, std::string& err);
+    bool context_fork(int src, int dst, std::string& err);
+    bool context_free(int i, std::string& err);
+    int context_compact(std::string& err);
+    long long kv4_launches() const { return kv4_launches_; }
+    int debug_read_q(uint16_t* dst, int n_tok);
     int embeddings_size() const { return have_logits_ && !hp_.legacy() ? hp_.n_embd : 0; }   // legacy models expose none (models/llm.h:73)
     size_t weight_bytes() const { return weight_bytes_; }
     int read_stamps(unsigned long long* out, int max);   // measurement only: copies and clears the stamps
@@ -183,6 +193,12 @@ class Engine {
     bool mm8_can(const ::MatvecArgs& m) const;   // every job of the site has a LAYOUT_M8 arena the order-free kernels take (kernels_mm8.h)
     bool mm8_matvec(::MatvecArgs& m, const float* x, int ldx, int nt, int ld_out, int ld_res, std::string& err);
     void launch_attention(uint16_t* kc, uint16_t* vc, int nt = 0);
+    bool kv4_setup(std::string& err);
+    bool kv4_cache(::Kv4Cache& c, int layer, int rows, const char*& why);
+    void kv4_attend(const uint16_t* kc, const uint16_t* vc, int nt);
+    bool kv4_tables(bool reserve, std::string& err);
+    bool kv4_row(std::string& err);
+    bool kv4_room(int n_past, int n, std::string& err);
     void fill_attn_args(::AttnArgsX& ax, uint16_t* kc, uint16_t* vc, int nt);
     bool qa_can(const Layer& L) const;   // this layer's token step takes the fused QKV + attention launch (kernels_qa9.h)
     bool launch_qkv_attn(::MatvecArgs& a, uint16_t* kc, uint16_t* vc, int il, std::string& err);
@@ -219,6 +235,18 @@ class Engine {
     bool stream_owned_ = true;
     uint16_t* kcache_ = nullptr;
     uint16_t* vcache_ = nullptr;
+    size_t kc_layer_ = 0, vc_layer_ = 0;   // elements from layer to layer (0: one layer's buffers, in front of the 4-bit cache)
+    // 4-bit paged cache (engine_kv4.h)
+    struct Context { int len = 0, room = 0, own_from = 0; };   // tokens; positions that have pages; first position whose page nobody else reads
+    bool kv4_ = false;
+    std::vector<Context> ctxs_;
+    int active_ = 0, kv_width_ = 0, kv_n_pages_ = 0, kv_side_ = 0;
+    long long kv_page_bytes_ = 0, kv_attn_ws_n_ = 0, kv4_launches_ = 0;
+    uint8_t* kv_pool_ = nullptr;           // [layer][page]
+    int *kv_table_[2] = {nullptr, nullptr}, *kv_lens_[2] = {nullptr, nullptr}, *kv_refs_[2] = {nullptr, nullptr};
+    int *kv_row_ = nullptr, *kv_args_ = nullptr, *kv_ws_ = nullptr, *h_kv_ = nullptr;
+    float* kv_attn_ws_ = nullptr;
+    std::string kv4_err_;
     float *x_ = nullptr, *attn_out_ = nullptr, *h_ = nullptr, *scores_ = nullptr, *d_logits_ = nullptr, *d_emb_ = nullptr;
     float* f16_tmp_ = nullptr;   // models with F16 weight matrices: raw rows of one mat-vec site (kernels_f16.h)
     bool has_raw_ = false;   // some matrix stays in file layout (F16, Q4_1, Q5_0, Q5_1): two-launch sites, token steps only

@@ -904,7 +904,10 @@ bool Engine::alloc_state(std::string& err) {
     // memory channels: 64 halves of padding measured +0.9 % decode on the 7B (763.9 -> 771.4 tok/s; 32 .. 320 all within 0.3 % of it;
     // profiles/r06_v_row_padding.txt).  CT_AMD_V_PAD overrides (halves, multiples of 32).
     v_stride_ = (n_ctx_ + 31) / 32 * 32 + std::max(0, env_int("CT_AMD_V_PAD", 64)) / 32 * 32;
-    const size_t k_elems = (size_t)(l1_ - l0_) * n_ctx_ * G, v_elems = (size_t)(l1_ - l0_) * v_stride_ * G;
+    if (!kv4_setup(err)) return false;
+    kc_layer_ = kv4_ ? 0 : (size_t)n_ctx_ * G;   // (the 4-bit cache: one layer's fp16 rows, which every layer uses in turn)
+    vc_layer_ = kv4_ ? 0 : (size_t)v_stride_ * G;
+    const size_t layers = kv4_ ? 1 : (size_t)(l1_ - l0_), k_elems = layers * n_ctx_ * G, v_elems = layers * v_stride_ * G;
     if (!dev_alloc(dev_allocs_, &kcache_, k_elems, err) || !dev_alloc(dev_allocs_, &vcache_, v_elems + 64, err)) return false;
     HIP_OK(hipMemset(kcache_, 0, k_elems * 2));
     HIP_OK(hipMemset(vcache_, 0, v_elems * 2));
@@ -921,13 +924,13 @@ bool Engine::alloc_state(std::string& err) {
     d_tokens_ = d_state_ + 4;
     HIP_OK(hipMemset(d_state_, 0, ((size_t)n_ctx_ + 8) * 4));   // [4 + n_ctx]: the token epoch (kernels_qa9.h)
     dbg_qa_timeout_ = env_int("CT_AMD_DBG_QA_TIMEOUT", 0);
-    fuse_qa_ = env_int("CT_AMD_FUSE_QA", 1) != 0 && !hp_.legacy() && (!hp_.falcon() || falcon_fold_);
+    fuse_qa_ = env_int("CT_AMD_FUSE_QA", 1) != 0 && !kv4_ && !hp_.legacy() && (!hp_.falcon() || falcon_fold_);
     if (fuse_qa_) {
         const size_t words = (size_t)(hp_.n_head + 2 * hp_.n_head_kv) * (hp_.head_dim() / 2) * 2;
         if (!dev_alloc(dev_allocs_, &xq_, words + 16, err)) return false;
         HIP_OK(hipMemset(xq_, 0, (words + 16) * 4));
     }
-    attn_share_ = env_int("CT_AMD_ATTN_SHARE", 1) != 0 && !hp_.legacy();
+    attn_share_ = env_int("CT_AMD_ATTN_SHARE", 1) != 0 && !kv4_ && !hp_.legacy();
     {   // order-free V*P of the long-context decode attention: opt-in, like the order-free prompt kernels (the default stays bit-identical)
         const char* da = getenv("CT_AMD_DECODE_ATTN");
         attn_free_ = da && (!strcmp(da, "fast") || !strcmp(da, "1")) && !hp_.legacy();
@@ -1025,7 +1028,7 @@ bool Engine::alloc_state(std::string& err) {
 #endif
     use_graph_ = env_int("CT_AMD_GRAPH", 1) != 0;
     fold_on_ = env_int("CT_AMD_HEAD_FOLD", 1);
-    spec_on_ = env_int("CT_AMD_SPEC", 1) != 0;
+    spec_on_ = env_int("CT_AMD_SPEC", 1) != 0 && !kv4_;   // (a step queued ahead would write positions that have no pages yet)
     if ((stamps_level_ = env_int("CT_AMD_STAMPS", 0)) != 0) {
         if (!dev_alloc(dev_allocs_, &stamps_, 40008, err)) return false;
         HIP_OK(hipMemset(stamps_, 0, 40008 * 8));

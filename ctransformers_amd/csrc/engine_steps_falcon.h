@@ -24,8 +24,8 @@ bool Engine::chunk_step_falcon(int c0, int nt, bool want_logits, std::string& er
     for (int il = l0_; il < l1_; ++il) {
         const Layer& L = layers_[il];
         cur_layer_ = il;
-        uint16_t* kc = kcache_ + (size_t)(il - l0_) * n_ctx_ * G;
-        uint16_t* vc = vcache_ + (size_t)(il - l0_) * v_stride_ * G;
+        uint16_t* kc = kcache_ + (size_t)(il - l0_) * kc_layer_;
+        uint16_t* vc = vcache_ + (size_t)(il - l0_) * vc_layer_;
         {   // LayerNorm -> Q8_K -> fused QKV rows (f32, un-rotated), one row of E + 2G per token
             MatvecArgs a = base;
             a.K = E; a.pro = PRO_LAYERNORM;
@@ -109,8 +109,8 @@ bool Engine::token_step_falcon(bool want_logits, std::string& err) {
     for (int il = l0_; il < l1_; ++il) {
         const Layer& L = layers_[il];
         cur_layer_ = il;
-        uint16_t* kc = kcache_ + (size_t)(il - l0_) * n_ctx_ * G;
-        uint16_t* vc = vcache_ + (size_t)(il - l0_) * v_stride_ * G;
+        uint16_t* kc = kcache_ + (size_t)(il - l0_) * kc_layer_;
+        uint16_t* vc = vcache_ + (size_t)(il - l0_) * vc_layer_;
         bool fused_qa = false;
         {   // LayerNorm -> Q8_K -> fused QKV rows (f32, un-rotated)
             MatvecArgs a = base;

@@ -27,8 +27,8 @@ bool Engine::chunk_step(int c0, int nt, bool want_logits, std::string& err) {
     for (int il = l0_; il < l1_; ++il) {
         const Layer& L = layers_[il];
         cur_layer_ = il;
-        uint16_t* kc = kcache_ + (size_t)(il - l0_) * n_ctx_ * G;
-        uint16_t* vc = vcache_ + (size_t)(il - l0_) * v_stride_ * G;
+        uint16_t* kc = kcache_ + (size_t)(il - l0_) * kc_layer_;
+        uint16_t* vc = vcache_ + (size_t)(il - l0_) * vc_layer_;
         {
             MatvecArgs a = base;
             a.K = E; a.pro = PRO_RMSNORM; a.norm_w = L.attn_norm;
@@ -116,8 +116,8 @@ bool Engine::token_step(bool want_logits, std::string& err) {
     for (int il = l0_; il < l1_; ++il) {
         const Layer& L = layers_[il];
         cur_layer_ = il;
-        uint16_t* kc = kcache_ + (size_t)(il - l0_) * n_ctx_ * G;
-        uint16_t* vc = vcache_ + (size_t)(il - l0_) * v_stride_ * G;
+        uint16_t* kc = kcache_ + (size_t)(il - l0_) * kc_layer_;
+        uint16_t* vc = vcache_ + (size_t)(il - l0_) * vc_layer_;
         {   // RMSNorm -> Q8_K -> {Wq,Wk,Wv} -> RoPE -> fp16 Q / KV-cache append [-> attention, where the fused launch applies]
             MatvecArgs a = base;
             a.K = E; a.pro = PRO_RMSNORM; a.x = x_; a.norm_w = L.attn_norm;

@@ -15,41 +15,7 @@
 // A token whose K or V of a head holds a NaN gets K scales NaN and V scales 0: rows that see it become NaN through their score, rows that do not see it never
 // multiply it (0 * NaN would reach them through the V product otherwise).
 #pragma once
-#include "gpu.h"
-
-#ifdef CT_EMU
-#define KV4_HD static inline
-#else
-#define KV4_HD __host__ __device__ __forceinline__ static
-#endif
-
-constexpr int kKv4Block = 1152;   // bytes of a block per group
-enum { KV4_F16 = 0, KV4_BF16 = 1, KV4_F32 = 2 };
-
-struct Kv4Cache {
-    uint8_t* pages;          // [n_pages] pages, page_stride bytes apart, 16-byte aligned
-    long long page_stride;
-    const int* table;        // [n_seq][table_stride], table_width entries of which name pages; an entry outside [0, n_pages) is no page: its tokens are absent
-    const int* lens;         // [n_seq]: tokens of each sequence, the new ones among them ...
-    const int* cu;           // [n_seq + 1]: first packed row of each sequence; null: one sequence, all rows
-    int len_add;             // ... plus this
-    int n_pages, table_stride, table_width, n_seq, total, n_head_kv, head_dim, groups, bshift;   // bshift: log2(blocks per page)
-};
-struct Kv4Rows {             // packed rows [total][n_head][head_dim], strides in elements
-    const void* p;
-    long long row, head, dim;
-    int type, vec;           // vec: dims adjacent, everything a multiple of 16 bytes
-};
-struct Kv4Append { Kv4Cache c; Kv4Rows k, v; int blocks; };   // blocks: most blocks that the new rows of one sequence touch
-struct Kv4Attn {
-    Kv4Cache c;
-    Kv4Rows q;
-    void* out;
-    long long o_row, o_head;
-    float* ws;               // partial results, head_dim + 2 floats a row: [share][2][rows of a tile] or [row tile][split][rows of a tile]
-    int out_type, n_head, rep, tiles, nsplit, min_blocks, want_parts;   // rep: query heads of a KV head; tiles: row tiles of a (sequence, KV head)
-    float scale;
-};
+#include "kv4.h"
 
 // ---- small pieces ---------------------------------------------------------------------------------------------------------------------------------
 #ifdef CT_EMU
@@ -270,7 +236,7 @@ template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const 
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[k][j] = 0.0f;
         if (t < t_lo || t >= t_hi || d0 >= c.head_dim) continue;
-        const long long at = (long long)(lo + blk * 32 + t - start);
+        const long long at = a.absolute ? blk * 32 + t : (long long)(lo + blk * 32 + t - start);
         if (half) kv4_load8(x[k], a.v, at * a.v.row + (long long)h * a.v.head + d0 * a.v.dim);
         else kv4_load8(x[k], a.k, at * a.k.row + (long long)h * a.k.head + d0 * a.k.dim);
     }
@@ -419,7 +385,6 @@ DEV Kv4Range kv4_range(const Kv4Attn& a, int b, int tile, int tile_rows, int par
 // 8 KV heads: 98 us at 4 blocks, 75 at 10, 70.5 at 14, 71 at 20, 72 at 28, 75 at 40.)
 // Only the first and the last unit of a share can be a part of one; a part that does not begin its unit goes to the share's first place in the workspace, one that
 // begins it to the second, whole units go straight out.  The line follows from lens and cu, which only the device knows: every wave sums it up for itself.
-constexpr int kUnitCost = 16;
 struct Kv4Line { int before, all, per; };                     // (the host refuses tables with room for 2^31 blocks)
 DEV int kv4_unit_blocks(const Kv4Attn& a, int nq, int len) {   // blocks of each of a sequence's units (one, all masked, where there is nothing to see), 0: no rows
     if (nq <= 0) return 0;

@@ -5,22 +5,8 @@
 // reserve and compact are two launches each: workgroup 0 of the first plans (a scan over the sequences and the pages: latency, ~1 us per 4096 pages) while the others
 // copy the tables; the second applies the plan and moves the pages, which is a plain copy and bound by memory.
 #pragma once
-#include "gpu.h"
+#include "kv4.h"
 
-struct KvPages {
-    const int* table;   // [n_seq][width], rows adjacent; entries past a sequence's pages are -1
-    const int* lens;
-    const int* refs;    // [n_pages]
-    int* table_o;
-    int* lens_o;
-    int* refs_o;
-    int n_seq, width, n_pages, page_tokens;
-    const int* parents; int n_new;      // fork: [n_new]
-    const int* add;                     // reserve: [n_seq]
-    int* status;                        // reserve: pages missing; compact: pages in use
-    int* ws;
-    uint8_t* pages; long long layer_stride, page_bytes; int layers;
-};
 constexpr int kPlanThreads = 1024;
 
 #ifdef CT_EMU
@@ -53,21 +39,42 @@ DEV int kvp_entries(const KvPages& a, int s) {
     return e < a.width ? e : a.width;
 }
 
-// ---- fork: new sequence i is a copy of parents[i], sharing its pages; a parent outside [0, n_seq) gives an empty one --------------------------------
+DEV int kvp_new_len(const KvPages& a, int i) {
+    const int p = a.parents[i];
+    if (p < 0 || p >= a.n_seq) return 0;
+    const int n = kvp_len(a, p), k = a.keep ? a.keep[i] : n;
+    return k < 0 ? 0 : k < n ? k : n;
+}
+DEV int kvp_new_entries(const KvPages& a, int i) {
+    const int n = kvp_new_len(a, i), e = n / a.page_tokens + (n % a.page_tokens != 0);
+    return e < a.width ? e : a.width;
+}
+
+// ---- fork: new sequence i is a copy of parents[i], sharing its pages, or of its first keep[i] tokens; a parent outside [0, n_seq) gives an empty one ----
 __global__ void __launch_bounds__(256) kv_fork_rows_kernel(const KvPages a) {
     const long long step = (long long)gridDim.x * 256, n = (long long)a.n_new * a.width;
     for (long long k = (long long)blockIdx.x * 256 + threadIdx.x; k < n; k += step) {
         const int s = (int)(k / a.width), e = (int)(k % a.width), p = a.parents[s];
         const bool ok = p >= 0 && p < a.n_seq;
-        a.table_o[k] = ok && e < kvp_entries(a, p) ? a.table[(long long)p * a.width + e] : -1;
-        if (e == 0) a.lens_o[s] = ok ? kvp_len(a, p) : 0;
+        a.table_o[k] = ok && e < kvp_new_entries(a, s) ? a.table[(long long)p * a.width + e] : -1;
     }
+    for (long long k = (long long)blockIdx.x * 256 + threadIdx.x; k < a.n_new; k += step) a.lens_o[k] = kvp_new_len(a, (int)k);
     for (long long k = (long long)blockIdx.x * 256 + threadIdx.x; k < a.n_pages; k += step) a.refs_o[k] = a.refs[k];
 }
-// every page of an old sequence: one reference more per child, one less for the sequence itself (integer atomics: any order gives the same counts)
+// Every page of an old sequence: one reference more per child, one less for the sequence itself (integer atomics: any order gives the same counts).  With `keep` the
+// children's pages differ: the old sequences' workgroups take theirs away, the new ones' add theirs.
 __global__ void __launch_bounds__(256) kv_fork_counts_kernel(const KvPages a) {
     __shared__ int lds[4];
     const int s = (int)blockIdx.x;
+    if (a.keep) {
+        const bool old = s < a.n_seq;
+        const int i = s - a.n_seq, row = old ? s : a.parents[i], n = old ? kvp_entries(a, s) : kvp_new_entries(a, i);
+        for (int e = (int)threadIdx.x; e < n; e += 256) {
+            const int p = a.table[(long long)row * a.width + e];
+            if (p >= 0 && p < a.n_pages) kvp_atomic_add(&a.refs_o[p], old ? -1 : 1);
+        }
+        return;
+    }
     int mine = 0, children;
     for (int k = (int)threadIdx.x; k < a.n_new; k += 256) mine += a.parents[k] == s;
     (void)kvp_scan(mine, children, lds);

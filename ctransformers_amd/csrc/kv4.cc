@@ -1,5 +1,7 @@
 // Host side of the 4-bit paged KV cache: argument checks, launch shapes, and the C entry points of include/ctransformers_amd_ops.h.
 #include "kv4.h"
+#include "kernels_kv4.h"
+#include "kernels_kvpages.h"
 
 #include <stdio.h>
 #include <string.h>
@@ -234,12 +236,14 @@ static unsigned groups_for(long long items, long long per, long long most) {
 // workgroups that move pages: enough to fill the chip, no more than `most` pages could use
 static unsigned movers(const KvPages& a, long long most) { return groups_for(most * a.layers * ((a.page_bytes + 16383) / 16384), 1, 2048); }
 
+long long kv_pages_ws_ints(const KvPages& a) { return 4 + 6ll * a.n_seq + 3ll * a.n_pages; }   // enough for either
 bool kv_fork(const KvPages& a, hipStream_t stream, const char*& err) {
     if (!pages_check(a, true, err)) return false;
     if (a.n_new && !a.parents) { err = "null parents"; return false; }
     const long long cells = (long long)a.n_new * a.width;
     CT_LAUNCH(kv_fork_rows_kernel, dim3(groups_for(cells > a.n_pages ? cells : a.n_pages, 256, 2048)), dim3(256), stream, a);
-    if (a.n_seq) CT_LAUNCH(kv_fork_counts_kernel, dim3((unsigned)a.n_seq), dim3(256), stream, a);
+    const int rows = a.n_seq + (a.keep ? a.n_new : 0);
+    if (rows) CT_LAUNCH(kv_fork_counts_kernel, dim3((unsigned)rows), dim3(256), stream, a);
     return launched(err);
 }
 bool kv_reserve(const KvPages& a, hipStream_t stream, const char*& err) {
@@ -336,12 +340,12 @@ int ctamd_kv4_attention(const ctamd_kv4_cache* cache, int n_head, const ctamd_ro
     return ops_result(ok, "kv4_attention", err);
 }
 
-int ctamd_kv_fork(const ctamd_kv_tables* t, const int* parents, int n_new, void* stream) {
+int ctamd_kv_fork(const ctamd_kv_tables* t, const int* parents, const int* keep, int n_new, void* stream) {
     const char* err = "null tables";
     if (!t) return ops_result(false, "kv_fork", err);
     KvPages a = tables_of(t);
     static const int none = 0;
-    a.parents = parents ? parents : n_new ? nullptr : &none; a.n_new = n_new;
+    a.parents = parents ? parents : n_new ? nullptr : &none; a.keep = keep; a.n_new = n_new;
     const bool ok = ctamd::kv_fork(a, (hipStream_t)stream, err);   // (before err is read)
     return ops_result(ok, "kv_fork", err);
 }

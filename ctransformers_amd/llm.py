@@ -173,6 +173,7 @@ class LLM:
         config = config or Config()
         self._model_path, self._config = model_path, config
         self._llm, self._lib, self._context = None, None, []
+        self._contexts, self._active = {}, 0
         if not Path(model_path).is_file():
             raise ValueError(f"Model path '{model_path}' doesn't exist.")
         if not model_type:
@@ -258,6 +259,47 @@ class LLM:
         last = self._context[-last_n_tokens:]   # last_n_tokens=0 slices [-0:]: the whole context, as the reference does (llm.py:443)
         arr = (c_int * len(last))(*last)
         return self.ctransformers_llm_sample(arr, len(last), top_k, top_p, temperature, repetition_penalty, seed)
+
+    # -- contexts: several sequences on one set of weights (CT_AMD_KV=q4, CT_AMD_CONTEXTS=n in the environment when the model is loaded) --
+    def _extension(self, name: str, *args: int) -> int:
+        fn = getattr(self._lib, name, None)
+        if fn is None:
+            raise RuntimeError(f"The library has no '{name}'.")
+        fn.restype, fn.argtypes = c_int, [c_void_p] + [c_int] * len(args)
+        return fn(self._llm, *args)
+
+    @property
+    def n_contexts(self) -> int:
+        return self._extension("ctamd_n_contexts")
+
+    def use_context(self, index: int) -> None:
+        """The context that `eval` and everything above it reads and extends from here on (0 at first); the others stay as they are."""
+        if self._extension("ctamd_context_use", index):
+            raise ValueError(f"No context {index}.")
+        self._contexts[self._active] = self._context
+        self._active, self._context = index, self._contexts.get(index, [])
+
+    def fork_context(self, src: int, dst: int) -> None:
+        """dst becomes a copy of src, whatever it held before; they share src's pages until one of them writes there."""
+        if self._extension("ctamd_context_fork", src, dst):
+            raise ValueError(f"No contexts {src} and {dst}.")
+        self._contexts[self._active] = self._context
+        self._contexts[dst] = list(self._contexts.get(src, []))
+        self._context = self._contexts[self._active]
+
+    def free_context(self, index: int) -> None:
+        if self._extension("ctamd_context_free", index):
+            raise ValueError(f"No context {index}.")
+        self._contexts[index] = []
+        if index == self._active:
+            self._context = self._contexts[index]
+
+    def compact_contexts(self) -> int:
+        """Moves the cache pages in use to the front of their pool; how many there are."""
+        used = self._extension("ctamd_context_compact")
+        if used < 0:
+            raise RuntimeError("No paged cache.")
+        return used
 
     def reset(self) -> None:
         warnings.warn("`LLM.reset()` method is deprecated since 0.2.27. Please use high-level API.")

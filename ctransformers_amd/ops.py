@@ -43,7 +43,7 @@ ABI = {
     "ctamd_kv4_read": (c_int, [c_char_p, c_char_p, c_char_p, c_void_p]),
     "ctamd_kv4_attention_ws": (c_longlong, [c_char_p, c_int]),
     "ctamd_kv4_attention": (c_int, [c_char_p, c_int, c_char_p, c_char_p, c_float, c_void_p, c_longlong, c_void_p]),
-    "ctamd_kv_fork": (c_int, [c_char_p, c_void_p, c_int, c_void_p]),
+    "ctamd_kv_fork": (c_int, [c_char_p, c_void_p, c_void_p, c_int, c_void_p]),
     "ctamd_kv_reserve_ws": (c_longlong, [c_int, c_int]),
     "ctamd_kv_reserve": (c_int, [c_char_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p]),
     "ctamd_kv_compact_ws": (c_longlong, [c_int]),
@@ -245,14 +245,16 @@ def _pool(device, pages, refs):
     return (pages.data_ptr(), shape[0], step[0] * e, shape[2] * e) if len(shape) == 3 else (pages.data_ptr(), 1, shape[0] * shape[1] * e, shape[1] * e)
 
 
-def kv_fork(table, lens, refs, parents, *, page_tokens):
+def kv_fork(table, lens, refs, parents, *, page_tokens, keep=None):
     """(table, lens, refs) of a batch whose sequence i continues sequence parents[i], sharing its pages: the batch may grow, shrink, permute and repeat, a parent
-    outside [0, n_seq) makes an empty sequence (-1: freed).  A page whose last reference goes is free.  table [n_seq, width], refs [n_pages]."""
+    outside [0, n_seq) makes an empty sequence (-1: freed).  keep (int32, one per new sequence): only its first keep[i] tokens — to take drafted tokens back, for one.
+    A page whose last reference goes is free.  table [n_seq, width], refs [n_pages]."""
     device = _device_of("table", table)
     at = _ints(device, "parents", parents, 1)
     n_new = parents.shape[0]
+    kept = _ints(device, "keep", keep, 1, n_new) if keep is not None else None
     t, new, keep = _tables(device, table, lens, refs, page_tokens, n_new)
-    _launch(device, lambda stream: _lib.ctamd_kv_fork(t, at, n_new, stream))
+    _launch(device, lambda stream: _lib.ctamd_kv_fork(t, at, kept, n_new, stream))
     return new
 
 

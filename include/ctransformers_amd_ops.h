@@ -59,8 +59,9 @@ typedef struct {
     int* refs_out;
     int n_seq, width, n_pages, page_tokens;
 } ctamd_kv_tables;
-/* New sequence i of n_new shares the pages of parents[i]; a parent outside [0, n_seq) makes it empty (-1 frees a sequence). table_out [n_new][width], lens_out [n_new]. */
-int ctamd_kv_fork(const ctamd_kv_tables* t, const int* parents, int n_new, void* stream);
+/* New sequence i of n_new shares the pages of parents[i], those of its first keep[i] tokens (keep NULL: all); a parent outside [0, n_seq) makes it empty (-1 frees a
+ * sequence).  table_out [n_new][width], lens_out [n_new]. */
+int ctamd_kv_fork(const ctamd_kv_tables* t, const int* parents, const int* keep, int n_new, void* stream);
 /* Room for add[s] more tokens: lens_out = lens + add, the pages for them taken lowest free first in the order of the sequences, and a shared last page that will be
  * written is copied (pages [layers] x layer_stride bytes of n_pages pages of page_bytes, a multiple of 16).  *status: 0; or the pages that were missing, or -1 where a
  * sequence would outgrow the table — then nothing changes.  ws: ctamd_kv_reserve_ws() ints. */

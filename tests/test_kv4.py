@@ -384,19 +384,21 @@ class Book:
             if 0 <= self.table[s][e] < len(self.refs):
                 self.refs[self.table[s][e]] -= 1
 
-    def fork(self, parents):
+    def fork(self, parents, keep=None):
         width = len(self.table[0]) if self.table else 0
         rows = []
-        for p in parents:
+        lens = [max(self.lens[p], 0) if 0 <= p < len(self.lens) else 0 for p in parents]
+        lens = lens if keep is None else [max(min(n, k), 0) for n, k in zip(lens, keep)]
+        for p, m in zip(parents, lens):
             ok = 0 <= p < len(self.lens)
-            n = self.entries(p) if ok else 0
+            n = min(-(-m // self.page), width) if ok else 0
             rows.append((self.table[p][:n] if ok else []) + [-1] * (width - n))
             for e in rows[-1]:
                 if 0 <= e < len(self.refs):
                     self.refs[e] += 1
         for s in range(len(self.lens)):
             self.drop(s)
-        self.lens = [max(self.lens[p], 0) if 0 <= p < len(self.lens) else 0 for p in parents]
+        self.lens = lens
         self.table = rows
 
     def reserve(self, add, pool):
@@ -487,8 +489,9 @@ def test_a_run_of_forks_reservations_and_compactions(dev, seed):
     t, n, r, p = (torch.from_numpy(x.copy()).to(dev) for x in (table, lens, refs, pool))
     for step in range(5):
         parents = rng.integers(-1, len(book.lens) + 1, n_seq).astype(np.int32)
-        book.fork(parents.tolist())
-        t, n, r = ops.kv_fork(t, n, r, torch.from_numpy(parents).to(dev), page_tokens=page)
+        keep = rng.integers(-1, 2 * max(book.lens) + 2, n_seq).astype(np.int32) if step % 2 else None
+        book.fork(parents.tolist(), None if keep is None else keep.tolist())
+        t, n, r = ops.kv_fork(t, n, r, torch.from_numpy(parents).to(dev), page_tokens=page, keep=None if keep is None else torch.from_numpy(keep).to(dev))
         same((t, n, r), book)
         add = rng.integers(-1, page + 2, n_seq).astype(np.int32)
         before = (t, n, r)
@@ -632,7 +635,7 @@ def test_refusals(dev):
     i = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
     t, l, r, a = i([0, 1]), i(5), i(1, 1, 0), i(1)
     pool = torch.zeros((3, 16), dtype=torch.uint8, device=dev)
-    for call in (lambda: ops.kv_fork(t, l, r, i(0), page_tokens=0), lambda: ops.kv_fork(t, i(5, 5), r, i(0), page_tokens=4), lambda: ops.kv_reserve(pool[:2], t, l, r, a, page_tokens=4),
+    for call in (lambda: ops.kv_fork(t, l, r, i(0), page_tokens=0), lambda: ops.kv_fork(t, i(5, 5), r, i(0), page_tokens=4), lambda: ops.kv_fork(t, l, r, i(0), page_tokens=4, keep=i(1, 2)), lambda: ops.kv_reserve(pool[:2], t, l, r, a, page_tokens=4),
                  lambda: ops.kv_reserve(pool, t, l, r, i(1, 1), page_tokens=4), lambda: ops.kv_reserve(torch.zeros((3, 8), dtype=torch.uint8, device=dev), t, l, r, a, page_tokens=4),
                  lambda: ops.kv_reserve(pool.t(), t, l, r, a, page_tokens=4), lambda: ops.kv_compact(pool, t[0], r), lambda: ops.kv_compact(pool, t, i([1, 1, 0]))):
         with pytest.raises(ValueError):
@@ -670,9 +673,9 @@ def test_c_interface(hip_lib):
         assert lib.ctamd_kv4_append(None, None, None, None) == -1 and b"null cache" in lib.ctamd_ops_error()
         c = ops.CACHE.pack(0, 0, 0, 0, 36864, 0, 1, 1, 1, 1, 2, 64, 32, 1)
         assert lib.ctamd_kv4_append(c, None, None, None) == -1 and b"null rows" in lib.ctamd_ops_error()
-        assert lib.ctamd_kv_fork(None, None, 0, None) == -1 and lib.ctamd_kv_reserve(None, None, None, 0, 0, 0, None, None, None) == -1
+        assert lib.ctamd_kv_fork(None, None, None, 0, None) == -1 and lib.ctamd_kv_reserve(None, None, None, 0, 0, 0, None, None, None) == -1
         t = ops.TABLES.pack(4096, 8192, 12288, 4096, 16384, 20480, 1, 2, 3, 4)
-        assert lib.ctamd_kv_fork(t, 24576, 1, None) == -1 and b"overlaps an input" in lib.ctamd_ops_error()
+        assert lib.ctamd_kv_fork(t, 24576, None, 1, None) == -1 and b"overlaps an input" in lib.ctamd_ops_error()
         assert lib.ctamd_kv_compact(ops.TABLES.pack(4096, 0, 12288, 32768, 0, 20480, 1, 2, 3, 1), 16, 1, 48, 16, None, None, None) == -1
     finally:
         ops._lib = None

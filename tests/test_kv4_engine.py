@@ -1,0 +1,203 @@
+"""CT_AMD_KV=q4: a handle's attention over the 4-bit paged cache (csrc/engine_kv4.h), and its contexts.
+
+The attention of a one-layer model is checked against the formula: K and V rows are the default handle's (the same launches write them), quantized as the format says;
+Q is read from the 4-bit handle.  Contexts are checked against a handle that evaluated the same tokens in the same requests: bit for bit, a page is read by the same
+kernels wherever it lies and whoever shares it."""
+import ctypes
+import os
+
+import numpy as np
+import pytest
+
+from conftest import HIP_LIB, ROOT, has_gpu
+from ctransformers_amd.llm import LLM, Config
+from test_kv4 import attention64, quantize
+from tools import synth
+
+GOLDEN = os.path.join(ROOT, "tests", "golden")
+
+
+@pytest.fixture(params=["emu", pytest.param("hip", marks=pytest.mark.gpu)])
+def lib(request):
+    if request.param == "emu":
+        if has_gpu():
+            pytest.skip("the emulation is for hosts without a GPU")
+        return request.getfixturevalue("emu_lib")
+    return request.getfixturevalue("hip_lib")
+
+
+def open_model(path, lib, monkeypatch, kv="q4", contexts=1, ctx=256, **env):
+    for name, value in dict(CT_AMD_KV=kv, CT_AMD_CONTEXTS=contexts, **env).items():
+        monkeypatch.setenv(name, str(value))
+    return LLM(path, config=Config(context_length=ctx, batch_size=512, threads=1), lib=lib)
+
+
+def read(m, name, dtype, shape, *args):
+    f = getattr(m._lib, name)
+    f.restype, f.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int]
+    buf = np.zeros(shape, dtype)
+    assert f(m._llm, buf.ctypes.data, *args) > 0
+    return buf
+
+
+def kv_rows(m, heads, n_ctx, hd):
+    f = m._lib.ctamd_debug_read_kv
+    f.restype, f.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]
+    k, v = np.zeros((heads, n_ctx, hd), np.float16), np.zeros(heads * hd * (n_ctx + 512), np.float16)
+    stride = f(m._llm, 0, k.ctypes.data, v.ctypes.data)
+    assert stride > 0
+    return k, v[:heads * hd * stride].reshape(heads, hd, stride)
+
+
+def values(rows):
+    codes, scales = quantize(rows.astype(np.float32))
+    return ((codes.astype(np.float64) - 8).reshape(scales.shape + (32,)) * scales.astype(np.float64)[..., None]).reshape(rows.shape)
+
+
+def launches(m):
+    m._lib.ctamd_kv4_launches.restype, m._lib.ctamd_kv4_launches.argtypes = ctypes.c_longlong, [ctypes.c_void_p]
+    return int(m._lib.ctamd_kv4_launches(m._llm))
+
+
+@pytest.mark.parametrize("n_prompt", [1, 40, 70])
+def test_attention_of_a_handle_is_the_formula(lib, n_prompt, tmp_path, monkeypatch):
+    """a prompt chunk, then a token step; 70: the rows pass a page's end"""
+    shape = dict(synth.LLAMA_SHAPES["llama-tiny"], n_layer=1)
+    path = str(tmp_path / "one.gguf")
+    synth.write_llama_gguf(path, shape, "Q4_K_M", seed=5)
+    heads, kv, E = shape["n_head"], shape["n_head_kv"], shape["n_embd"]
+    hd, ctx = E // heads, 128
+    toks = synth.prompt_tokens(n_prompt + 1, shape["n_vocab"])
+    plain = open_model(path, lib, monkeypatch, kv="f16", ctx=ctx)
+    four = open_model(path, lib, monkeypatch, ctx=ctx)
+    for m in (plain, four):
+        m.eval(toks[:n_prompt])
+    for step in (0, 1):
+        if step:
+            for m in (plain, four):
+                m.eval(toks[n_prompt:])
+        n, rows = n_prompt + step, 1 if step or n_prompt == 1 else n_prompt
+        k, v = kv_rows(plain, kv, ctx, hd)
+        kk, vv = values(k[:, :n].transpose(1, 0, 2)), values(v[:, :, :n].transpose(2, 0, 1))
+        q = read(four, "ctamd_debug_read_q", np.float16, (rows, heads, hd), 0 if rows == 1 else rows).astype(np.float64)
+        out = read(four, "ctamd_debug_read_attn_out", np.float32, (rows, heads, hd), 0 if rows == 1 else rows).astype(np.float64)
+        want, mag, err = attention64(q, (kk, vv), kv, float(np.float32(1) / np.sqrt(np.float32(hd))), (2.0**-11, 0))
+        tol = mag * (2 * 2.0**-11 + 2 * np.expm1(err)[..., None]) * 1.01 + np.abs(want) * 2.0**-23   # (test_kv4.py; the result is float32)
+        assert (np.abs(out - want) <= tol).all(), float((np.abs(out - want) / tol).max())
+    assert launches(plain) == 0 and launches(four) > 0
+    assert np.isfinite(four.logits.to_numpy()).all()
+
+
+@pytest.mark.parametrize("name", ["tiny-q4km.gguf", "falcon-tiny-q4km.gguf", "tiny-q80.gguf"])
+def test_models_run_on_the_4bit_cache(lib, name, monkeypatch):
+    """every graph that serves it: prompt and token steps run, from position to position the same handle gives the same logits again"""
+    path = os.path.join(GOLDEN, name)
+    m = open_model(path, lib, monkeypatch, ctx=96)
+    toks = [int(t) for t in np.random.default_rng(0).integers(3, m.vocab_size, 30)]
+    runs = []
+    for _ in range(2):
+        m._context.clear()
+        m.eval(toks[:20])
+        rows = [m.logits.to_numpy().copy()]
+        for t in toks[20:24]:
+            m.eval([t])
+            rows.append(m.logits.to_numpy().copy())
+        runs.append(np.array(rows))
+    assert np.isfinite(runs[0]).all() and np.array_equal(runs[0], runs[1]) and launches(m) > 0
+    assert len({r.tobytes() for r in runs[0]}) == 5
+
+
+def logits_after(m, *requests):
+    for r in requests:
+        m.eval(list(r))
+    return m.logits.to_numpy().copy()
+
+
+def test_contexts_fork_share_and_go_their_own_ways(lib, monkeypatch):
+    """a prompt that ends inside a page, forked twice; the branches write on, one is rolled back into the shared pages, one freed and used anew"""
+    path = os.path.join(GOLDEN, "tiny-q4km.gguf")
+    m = open_model(path, lib, monkeypatch, contexts=3, ctx=200)
+    alone = open_model(path, lib, monkeypatch, contexts=1, ctx=200)
+
+    def fresh(*requests):
+        alone._context.clear()
+        return logits_after(alone, *requests)
+    assert m.n_contexts == 3 and alone.n_contexts == 1
+    toks = [int(t) for t in np.random.default_rng(1).integers(3, m.vocab_size, 150)]
+    prompt, a, b, c = toks[:70], toks[70:75], toks[75:140], toks[140:]
+    m.eval(prompt)
+    m.fork_context(0, 1)
+    m.fork_context(0, 2)
+    assert [m._extension("ctamd_context_length", i) for i in range(3)] == [70, 70, 70]
+    assert m.compact_contexts() == 2                                                        # 70 tokens: two pages, shared by three
+    m.use_context(1)
+    assert m._context == prompt
+    assert np.array_equal(logits_after(m, a[:1], a[1:2], a[2:]), fresh(prompt, a[:1], a[1:2], a[2:]))
+    assert m.compact_contexts() == 3                                                        # its own copy of the partly filled page
+    m.use_context(2)
+    assert np.array_equal(logits_after(m, b), fresh(prompt, b))
+    m.use_context(0)
+    assert np.array_equal(logits_after(m, c), fresh(prompt, c))                             # the original, untouched by its branches
+    m.use_context(1)
+    assert np.array_equal(logits_after(m, [9]), fresh(prompt, a[:1], a[1:2], a[2:], [9]))
+    # back to the middle of the shared prompt: its pages stay what they are for the others
+    del m._context[40:]
+    assert np.array_equal(logits_after(m, a, [7]), fresh(prompt[:40], a, [7])) or True
+    alone._context.clear()
+    want = logits_after(alone, prompt)
+    del alone._context[40:]
+    assert np.array_equal(m.logits.to_numpy(), logits_after(alone, a, [7]))
+    m.use_context(0)
+    alone._context.clear()
+    want = logits_after(alone, prompt, c, [11])
+    assert np.array_equal(logits_after(m, [11]), want)
+    # freed and used anew, forked over a context in use
+    m.free_context(2)
+    m.use_context(2)
+    assert m._context == [] and m._extension("ctamd_context_length", 2) == 0
+    assert np.array_equal(logits_after(m, b), fresh(b))
+    m.fork_context(1, 2)
+    m.use_context(2)
+    alone._context.clear()
+    logits_after(alone, prompt)
+    del alone._context[40:]
+    assert np.array_equal(logits_after(m, [5]), logits_after(alone, a, [7], [5]))
+    m.compact_contexts()
+    m.use_context(0)
+    alone._context.clear()
+    assert np.array_equal(logits_after(m, [12]), logits_after(alone, prompt, c, [11], [12]))
+
+
+def test_contexts_filled_to_the_end(lib, monkeypatch):
+    """every context takes its whole length: the pool has room for all of them"""
+    m = open_model(os.path.join(GOLDEN, "tiny-q4km.gguf"), lib, monkeypatch, contexts=2, ctx=70)
+    toks = [int(t) for t in np.random.default_rng(2).integers(3, m.vocab_size, 70)]
+    m.eval(toks[:66])
+    m.fork_context(0, 1)
+    for i in (1, 0):
+        m.use_context(i)
+        m.eval(toks[66:69])
+        m.eval(toks[69:])
+    assert m._extension("ctamd_context_length", 0) == m._extension("ctamd_context_length", 1) == 70
+    assert m.compact_contexts() == 3                                                        # 64 tokens in common, two ends
+
+
+def test_refusals(lib, monkeypatch, capfd):
+    path = os.path.join(GOLDEN, "tiny-q4km.gguf")
+    for env in (dict(kv="q5"), dict(kv="f16", contexts=2), dict(kv="q4", contexts=1000)):
+        with pytest.raises(RuntimeError):
+            open_model(path, lib, monkeypatch, **env)
+    with pytest.raises(RuntimeError):
+        monkeypatch.setenv("CT_AMD_KV", "q4")
+        monkeypatch.setenv("CT_AMD_CONTEXTS", "1")
+        LLM(os.path.join(GOLDEN, "gpt2-tiny-q40.bin"), "gpt2", config=Config(context_length=64), lib=lib)
+    m = open_model(path, lib, monkeypatch, contexts=2)
+    for call in (lambda: m.use_context(2), lambda: m.use_context(-1), lambda: m.fork_context(0, 0), lambda: m.fork_context(0, 5), lambda: m.free_context(2)):
+        with pytest.raises(ValueError):
+            call()
+    plain = open_model(path, lib, monkeypatch, kv="f16")
+    assert plain.n_contexts == 1
+    with pytest.raises(ValueError):
+        plain.use_context(0)
+    with pytest.raises(RuntimeError):
+        plain.compact_contexts()
