@@ -240,7 +240,7 @@ class Engine {
     struct Context { int len = 0, room = 0, own_from = 0; };   // tokens; positions that have pages; first position whose page nobody else reads
     bool kv4_ = false;
     std::vector<Context> ctxs_;
-    int active_ = 0, kv_width_ = 0, kv_n_pages_ = 0, kv_side_ = 0;
+    int active_ = 0, kv_page_ = 64, kv_width_ = 0, kv_n_pages_ = 0, kv_side_ = 0;
     long long kv_page_bytes_ = 0, kv_attn_ws_n_ = 0, kv4_launches_ = 0;
     uint8_t* kv_pool_ = nullptr;           // [layer][page]
     int *kv_table_[2] = {nullptr, nullptr}, *kv_lens_[2] = {nullptr, nullptr}, *kv_refs_[2] = {nullptr, nullptr};

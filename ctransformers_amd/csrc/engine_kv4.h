@@ -1,13 +1,11 @@
 // The 4-bit KV cache of a handle (CT_AMD_KV=q4) and its contexts (CT_AMD_CONTEXTS) — part of engine.cc, included there inside namespace ctamd.  Not a stand-alone header.
 //
 // The mat-vec launches leave fp16 K / V rows at their positions as without it, in buffers of ONE layer that all layers use in turn; behind them every layer quantizes
-// the new rows into its pages (kv4_append) and attends to the pages (kv4_attention), the new rows among them.  A page is 64 tokens of all KV heads of a layer; one
-// page table serves all layers.  A handle holds n contexts (sequences) on one set of weights: evals read and write the active one, a fork shares pages, and
+// the new rows into its pages (kv4_append) and attends to the pages (kv4_attention), the new rows among them.  A page is 64 tokens (CT_AMD_KV_PAGE: 32, 64, 128, 256) of all KV heads of a
+// layer; one page table serves all layers.  A handle holds n contexts (sequences) on one set of weights: evals read and write the active one, a fork shares pages, and
 // positions in shared pages are given pages of their own before they are written (kv_reserve copies a partly filled one).  The pool has room for every context's
 // full length, so making room never fails.  The tables change only where an eval enters positions without room of their own (once every 64 tokens of a plain
 // continuation): token steps replay their graphs, which read the active context's row of the table at a fixed address.
-
-constexpr int kKvPage = 64;
 
 bool Engine::kv4_setup(std::string& err) {
     const char* kind = getenv("CT_AMD_KV");
@@ -21,10 +19,11 @@ bool Engine::kv4_setup(std::string& err) {
     if (hp_.legacy() || l0_ != 0 || l1_ != hp_.n_layer) { err = "CT_AMD_KV=q4 serves llama and falcon models on one GPU"; return false; }
     if (n > 256) { err = "CT_AMD_CONTEXTS: at most 256"; return false; }
     ctxs_.assign((size_t)n, Context());
-    kv_width_ = (n_ctx_ + kKvPage - 1) / kKvPage;
+    kv_page_ = env_int("CT_AMD_KV_PAGE", 64);
+    kv_page_bytes_ = kv4_page_bytes(hp_.n_head_kv, hp_.head_dim(), kv_page_);
+    if (!kv_page_bytes_) { err = "CT_AMD_KV=q4: head size, or CT_AMD_KV_PAGE (32, 64, 128, 256), not supported"; return false; }
+    kv_width_ = (n_ctx_ + kv_page_ - 1) / kv_page_;
     kv_n_pages_ = n * kv_width_;
-    kv_page_bytes_ = kv4_page_bytes(hp_.n_head_kv, hp_.head_dim(), kKvPage);
-    if (!kv_page_bytes_) { err = "CT_AMD_KV=q4: head size not supported"; return false; }
     const size_t pool = (size_t)hp_.n_layer * kv_n_pages_ * kv_page_bytes_;
     if (!dev_alloc(dev_allocs_, &kv_pool_, pool, err)) return false;
     HIP_OK(hipMemset(kv_pool_, 0, pool));
@@ -59,7 +58,7 @@ bool Engine::kv4_cache(Kv4Cache& c, int layer, int rows, const char*& why) {
     c.len_add = rows;
     c.n_pages = kv_n_pages_; c.table_stride = c.table_width = kv_width_;
     c.n_seq = 1; c.total = rows; c.n_head_kv = hp_.n_head_kv; c.head_dim = hp_.head_dim();
-    return kv4_check(c, kKvPage, why);
+    return kv4_check(c, kv_page_, why);
 }
 
 // the layer's rows of this step from the fp16 buffers into its pages, then attention over the pages
@@ -93,7 +92,7 @@ bool Engine::kv4_tables(bool reserve, std::string& err) {
     KvPages a = KvPages();
     a.table = kv_table_[i]; a.lens = kv_lens_[i]; a.refs = kv_refs_[i];
     a.table_o = kv_table_[o]; a.lens_o = kv_lens_[o]; a.refs_o = kv_refs_[o];
-    a.n_seq = n; a.width = kv_width_; a.n_pages = kv_n_pages_; a.page_tokens = kKvPage;
+    a.n_seq = n; a.width = kv_width_; a.n_pages = kv_n_pages_; a.page_tokens = kv_page_;
     const char* why = nullptr;
     bool ok;
     if (reserve) {
@@ -131,10 +130,10 @@ bool Engine::kv4_room(int n_past, int n, std::string& err) {
         c.len = need;
         return true;
     }
-    const int end = std::min((need + kKvPage - 1) / kKvPage * kKvPage, kv_width_ * kKvPage);
+    const int end = std::min((need + kv_page_ - 1) / kv_page_ * kv_page_, kv_width_ * kv_page_);
     for (int i = 0; i < m; ++i) h_kv_[i] = i == active_ ? end - c.room : 0;
     if (!kv4_tables(true, err)) return false;
-    const int from = c.room / kKvPage * kKvPage;   // (a partly filled last page is the context's own now: reserve copied it if it was shared)
+    const int from = c.room / kv_page_ * kv_page_;   // (a partly filled last page is the context's own now: reserve copied it if it was shared)
     c.own_from = cut ? from : std::min(c.own_from, from);
     c.room = end;
     c.len = need;
@@ -154,7 +153,7 @@ bool Engine::context_fork(int src, int dst, std::string& err) {
     HIP_OK(hipSetDevice(device_));
     for (int i = 0; i < m; ++i) { h_kv_[i] = i == dst ? src : i; h_kv_[m + i] = i == dst ? ctxs_[src].len : 0x7FFFFFFF; }
     if (!kv4_tables(false, err)) return false;
-    const int len = ctxs_[src].len, shared = (len + kKvPage - 1) / kKvPage * kKvPage;
+    const int len = ctxs_[src].len, shared = (len + kv_page_ - 1) / kv_page_ * kv_page_;
     ctxs_[src].own_from = std::max(ctxs_[src].own_from, shared);
     ctxs_[dst] = Context{len, len, shared};
     return kv4_row(err);
@@ -174,7 +173,7 @@ int Engine::context_compact(std::string& err) {   // pages in use, -1: failed
     (void)hipSetDevice(device_);
     KvPages a = KvPages();
     a.table = kv_table_[i]; a.refs = kv_refs_[i]; a.table_o = kv_table_[o]; a.refs_o = kv_refs_[o];
-    a.n_seq = n; a.width = kv_width_; a.n_pages = kv_n_pages_; a.page_tokens = kKvPage;
+    a.n_seq = n; a.width = kv_width_; a.n_pages = kv_n_pages_; a.page_tokens = kv_page_;
     a.pages = kv_pool_; a.layers = hp_.n_layer; a.layer_stride = kv_n_pages_ * kv_page_bytes_; a.page_bytes = kv_page_bytes_;
     a.status = kv_args_ + 2 * n; a.ws = kv_ws_;
     const char* why = nullptr;
