@@ -455,7 +455,8 @@ DEV u32x4 kv4_values(uint32_t w, uint32_t s0, uint32_t s1, uint32_t s2, uint32_t
 //   O = V^T (A: lane = dim) x P (B: lane = row): those eight probabilities ARE the lane's k slots — V is stored in that order
 // K's codes enter as f16 SUBNORMALS, the 16-bit integers themselves (code * 2^-24: no conversion); -8 * sum(Q) is the product's C operand and the group's scale
 // multiplies the 32-dim product in f32, so K is used exactly.  Maximum, sum and O stay per lane in f32; the maximum is raised (and O rescaled) only when a score
-// passes it by more than 2^8, so most blocks exchange nothing between lanes (p <= 256 fits f16 as well as p <= 1 does).
+// passes it by more than 2^8, so most blocks exchange nothing between lanes (p <= 256 fits f16 as well as p <= 1 does).  P enters as two halves, the rounded one and
+// what it left (the matrix cores have the time: +2 % at most), so that what is rounded on the way is V's product with its scale alone.
 // The next block's K is fetched into the registers of this one's as soon as its scores are there, its V after the V product: 40 dwords a lane at 128 dims for a
 // block in flight, which leaves room for four waves a SIMD.
 template <int G> DEV void kv4_fetch_k(uint32_t (&kc)[2][G], uint32_t (&ks)[2][2 * G], const uint8_t* blk, int m, int i) {
@@ -600,7 +601,7 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
         }
         kv4_fetch_k<G>(kc, ks, nxt, m, i);
         {
-            u32x4 P[NT];
+            u32x4 P[NT], PL[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 if (p0 + 32 > free_lim || p0 + 32 > there) {
@@ -627,16 +628,17 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
                         for (int e = 0; e < 4; ++e) O[n][j][e] *= f;
                 }
                 const float base = mx[n] == -INFINITY ? 0.0f : -mx[n];
-                uint32_t pk[4];
+                uint32_t pk[4], lo[4];
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const float x = exp2_fast(fmaf(s[n][t][e], sc2[n], base)), y = exp2_fast(fmaf(s[n][t][e + 1], sc2[n], base));
-                        pk[2 * t + e / 2] = kv4_cvt2(x, y);   // the probabilities as halves: 2^-11 of each at most, independent of one another; their sum is of the halves
-                        sum[n] = kv4_sum2(pk[2 * t + e / 2], sum[n]);
-                    }
+                for (int p = 0; p < 4; ++p) {
+                    const float x = exp2_fast(fmaf(s[n][p / 2][2 * (p & 1)], sc2[n], base)), y = exp2_fast(fmaf(s[n][p / 2][2 * (p & 1) + 1], sc2[n], base));
+                    pk[p] = kv4_cvt2(x, y);
+                    sum[n] += x;
+                    sum[n] += y;
+                    lo[p] = kv4_cvt2(x - f16_bits_to_f32((uint16_t)(pk[p] & 0xFFFFu)), y - f16_bits_to_f32((uint16_t)(pk[p] >> 16)));
+                }
                 P[n] = u32x4_of(pk[0], pk[1], pk[2], pk[3]);
+                PL[n] = u32x4_of(lo[0], lo[1], lo[2], lo[3]);
             }
             if (p0 + 32 > there) {   // whatever the page holds past the sequence's end must not meet p = 0 as an infinity
 #pragma unroll
@@ -652,7 +654,10 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
                 const int s0 = j < 4 * (G / 2) ? 4 * (j / 4) : 2 * (G - 1);
                 const u32x4 v = kv4_values(vc[j], vs[s0], vs[s0 + 1], vs[s0 + 2], vs[s0 + 3]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) O[n][j] = mfma_f16_16x16x32(v, P[n], O[n][j]);
+                for (int n = 0; n < NT; ++n) {
+                    O[n][j] = mfma_f16_16x16x32(v, P[n], O[n][j]);
+                    O[n][j] = mfma_f16_16x16x32(v, PL[n], O[n][j]);
+                }
             }
         }
         kv4_fetch_v<G>(vc, vs, nxt, m, i);

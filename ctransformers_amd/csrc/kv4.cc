@@ -91,10 +91,13 @@ bool kv4_read(Kv4Append& a, int max_rows, hipStream_t stream, const char*& err) 
     return launched(err);
 }
 
-// Rows of a tile: kv4_decode_kernel takes 16 (32 where heads are small enough for two tiles in registers), kv4_prompt_kernel 128.
+// Rows of a tile: kv4_decode_kernel takes 16, or 32 where two tiles of a head fit the registers (128 dims), kv4_prompt_kernel 128.  The first streams the codes at
+// memory speed once per tile, the second unpacks them once for 128 rows but takes at least as long for fewer.  Measured, 16 sequences of up to 8000 tokens, 8 KV heads,
+// the first against the second, us: 128 dims 40 rows 42 / 77, 64 rows 50 / 80, 96 rows 63 / 83, 128 rows 82 / 91 (one sequence: 35 / 31, 400 tokens: 34 / 25);
+// 64 dims 64 rows 30 / 52, 96 rows 35 / 55, 128 rows 42 / 56, 256 rows 71 / 102.
 static int tile_rows(const Kv4Attn& a, long long rows) {
     if (rows <= 16) return 16;
-    if (rows <= 32 && a.c.groups <= 4) return 32;
+    if (a.c.groups <= 4 && rows <= (a.c.groups <= 2 ? 192 : 96)) return 32;
     return 128;
 }
 static int chip_cus() {   // of the current device; asked for once per device
