@@ -51,6 +51,8 @@ ABI = {
 }
 _lib = None
 _on_gpu = True
+# the address of a device's current stream without making a Stream object of it, where torch has that
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def load(path=None):
@@ -75,10 +77,10 @@ def _launch(device, fn):
     if device < 0:
         code = fn(None)
     elif device == torch.cuda.current_device():
-        code = fn(torch.cuda.current_stream(device).cuda_stream)
+        code = fn(_stream(device))
     else:
         with torch.cuda.device(device):
-            code = fn(torch.cuda.current_stream(device).cuda_stream)
+            code = fn(_stream(device))
     if code:
         raise ValueError(_lib.ctamd_ops_error().decode())
 
@@ -213,8 +215,8 @@ def kv4_attention(q, pages, table, lens, cu, max_rows, *, n_head_kv, page_tokens
     return out
 
 
-def _tables(device, table, lens, refs, page_tokens, rows=None):
-    """(the packed structure, outputs, what has to outlive the call)"""
+def _tables(device, table, lens, refs, page_tokens, rows=None, extra=0):
+    """(the packed structure, outputs, the extra ints, their address, what has to outlive the call)"""
     tp = _ints(device, "table", table, 2)
     n_seq, width = table.shape
     rp = _ints(device, "refs", refs, 1)
@@ -226,11 +228,13 @@ def _tables(device, table, lens, refs, page_tokens, rows=None):
         tp = table.data_ptr()
     if rows is None:
         rows = n_seq
-    on = refs.device
-    t = torch.empty((rows, width), dtype=_INT, device=on)
-    n = torch.empty((rows,), dtype=_INT, device=on) if lens is not None else None
-    r = torch.empty(refs.shape, dtype=_INT, device=on)
-    return TABLES.pack(tp, lp, rp, t.data_ptr(), n.data_ptr() if lens is not None else 0, r.data_ptr(), n_seq, width, refs.shape[0], page_tokens), (t, n, r), table
+    # the results are parts of one allocation, behind them `extra` ints (a status word and a workspace)
+    n_pages, cells = refs.shape[0], rows * width
+    both = torch.empty(cells + rows + n_pages + extra, dtype=_INT, device=refs.device)
+    t, n, r, more = both.split((cells, rows, n_pages, extra))
+    at = both.data_ptr()
+    ends = at + 4 * cells, at + 4 * (cells + rows), at + 4 * (cells + rows + n_pages)
+    return TABLES.pack(tp, lp, rp, at, ends[0] if lens is not None else 0, ends[1], n_seq, width, n_pages, page_tokens), (t.view(rows, width), n, r), more, ends[2], table
 
 
 def _pool(device, pages, refs):
@@ -253,7 +257,7 @@ def kv_fork(table, lens, refs, parents, *, page_tokens, keep=None):
     at = _ints(device, "parents", parents, 1)
     n_new = parents.shape[0]
     kept = _ints(device, "keep", keep, 1, n_new) if keep is not None else None
-    t, new, keep = _tables(device, table, lens, refs, page_tokens, n_new)
+    t, new, _, _, alive = _tables(device, table, lens, refs, page_tokens, n_new)
     _launch(device, lambda stream: _lib.ctamd_kv_fork(t, at, kept, n_new, stream))
     return new
 
@@ -263,24 +267,20 @@ def kv_reserve(pages, table, lens, refs, add, *, page_tokens):
     and a last page that others share is copied before its sequence writes it.  pages: [n_pages, ..] or [layers, n_pages, ..], any type.  short (int32, on the
     device): 0, or the pages that were missing, or -1 where a sequence outgrows its row of the table; then nothing has changed."""
     device = _device_of("table", table)
-    t, new, keep = _tables(device, table, lens, refs, page_tokens)
-    n_seq, n_pages = table.shape[0], refs.shape[0]
+    _ints(device, "refs", refs, 1)
+    n_seq = table.shape[0]
+    t, new, rest, sp, alive = _tables(device, table, lens, refs, page_tokens, None, 1 + _lib.ctamd_kv_reserve_ws(n_seq, refs.shape[0]))
     more = _ints(device, "add", add, 1, n_seq)
     at, layers, layer_bytes, page_bytes = _pool(device, pages, refs)
-    short = torch.empty((), dtype=_INT, device=refs.device)
-    ws = torch.empty(_lib.ctamd_kv_reserve_ws(n_seq, n_pages), dtype=_INT, device=refs.device)
-    sp, wp = short.data_ptr(), ws.data_ptr()
-    _launch(device, lambda stream: _lib.ctamd_kv_reserve(t, more, at, layers, layer_bytes, page_bytes, sp, wp, stream))
-    return new + (short,)
+    _launch(device, lambda stream: _lib.ctamd_kv_reserve(t, more, at, layers, layer_bytes, page_bytes, sp, sp + 4, stream))
+    return new + (rest[0],)
 
 
 def kv_compact(pages, table, refs):
     """(table, refs, used) after the pages in use have become pages 0 .. used - 1: those beyond move, in order, into the holes below.  used: int32, on the device."""
     device = _device_of("table", table)
-    t, new, keep = _tables(device, table, None, refs, 1)
+    _ints(device, "refs", refs, 1)
+    t, new, rest, up, alive = _tables(device, table, None, refs, 1, None, 1 + _lib.ctamd_kv_compact_ws(refs.shape[0]))
     at, layers, layer_bytes, page_bytes = _pool(device, pages, refs)
-    used = torch.empty((), dtype=_INT, device=refs.device)
-    ws = torch.empty(_lib.ctamd_kv_compact_ws(refs.shape[0]), dtype=_INT, device=refs.device)
-    up, wp = used.data_ptr(), ws.data_ptr()
-    _launch(device, lambda stream: _lib.ctamd_kv_compact(t, at, layers, layer_bytes, page_bytes, up, wp, stream))
-    return new[0], new[2], used
+    _launch(device, lambda stream: _lib.ctamd_kv_compact(t, at, layers, layer_bytes, page_bytes, up, up + 4, stream))
+    return new[0], new[2], rest[0]
