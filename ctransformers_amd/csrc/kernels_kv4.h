@@ -218,16 +218,22 @@ template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const 
     __shared__ uint16_t sc[2][32][G];
     __shared__ int poison[32];
     const Kv4Cache& c = a.c;
-    const int tid = (int)threadIdx.x, h = (int)blockIdx.y, b = (int)blockIdx.x / a.blocks;
+    const int tid = (int)threadIdx.x, h = (int)blockIdx.x % c.n_head_kv, place = (int)blockIdx.x / c.n_head_kv, b = place / a.blocks;   // (heads lie side by side in a row)
     int lo, hi, len;
     kv4_seq(c, b, lo, hi, len);
     const int start = len - (hi - lo);                          // position of the first new row (rows before position 0 are dropped)
-    const int blk = (start > 0 ? start : 0) / 32 + (int)blockIdx.x % a.blocks;
+    const int blk = (start > 0 ? start : 0) / 32 + place % a.blocks;
     if (blk * 32 >= len || hi == lo) return;
     uint8_t* dst = kv4_block(c, b, h, blk);
     if (!dst) return;
     const int t_lo = start > blk * 32 ? start - blk * 32 : 0, t_hi = len - blk * 32 < 32 ? len - blk * 32 : 32;   // the new tokens of this block
     if (tid < 32) poison[tid] = 0;
+    uint32_t* vd = (uint32_t*)(dst + 512 * G);
+    uint32_t old[(G + 1) / 2];   // the V dwords that keep older (or the neighbours of newer) tokens: fetched with the rows, not behind them
+    if (t_hi - t_lo < 32) {
+#pragma unroll
+        for (int k = 0; k < (G + 1) / 2; ++k) old[k] = tid + 256 * k < 4 * 32 * G ? vd[tid + 256 * k] : 0u;
+    }
     // piece `it` of 256 G: half (K, V), token, group, eight dims
     float x[G][8];
 #pragma unroll
@@ -245,6 +251,7 @@ template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const 
     for (int k = 0; k < G; ++k) {
         const int it = tid + 256 * k, half = it / (128 * G), t = (it / (4 * G)) & 31, g = (it / 4) % G, o = it & 3;
         const bool on = t >= t_lo && t < t_hi;
+        if (!__ballot(on)) continue;   // (a token step: one wave has work)
         float top = 0.0f;
         int nan = 0;
 #pragma unroll
@@ -294,9 +301,10 @@ template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const 
         if (half) s[(i * G + g) * 8 + (t & 3) + 4 * (t / 16)] = poison[t] ? (uint16_t)0 : sc[1][t][g];
         else s[(((t / 16) * 4 + i) * G + g) * 4 + (t & 3)] = poison[t] ? (uint16_t)0x7E00 : sc[0][t][g];
     }
-    uint32_t* vd = (uint32_t*)(dst + 512 * G);
-    for (int it = tid; it < 4 * 32 * G; it += 256) {
-        const int i = it / (32 * G), dim = it % (32 * G);
+#pragma unroll
+    for (int k = 0; k < (G + 1) / 2; ++k) {
+        const int it = tid + 256 * k, i = it / (32 * G), dim = it % (32 * G);
+        if (it >= 4 * 32 * G) break;
         uint32_t w = 0, m = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -305,18 +313,18 @@ template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const 
             w |= ((vcode[t][dim / 4] >> (8 * (dim & 3))) & 15u) << sh;
             m |= 15u << sh;
         }
-        if (m) vd[it] = m == 0xFFFFFFFFu ? w : (vd[it] & ~m) | w;
+        if (m) vd[it] = m == 0xFFFFFFFFu ? w : (old[k] & ~m) | w;
     }
 }
 
 // The last rows of every sequence out of the cache, as numbers: the mirror image of kv4_append_kernel, same workgroups.  Rows whose page is absent are zeros.
 template <int G> __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Append a) {
     const Kv4Cache& c = a.c;
-    const int tid = (int)threadIdx.x, h = (int)blockIdx.y, b = (int)blockIdx.x / a.blocks;
+    const int tid = (int)threadIdx.x, h = (int)blockIdx.x % c.n_head_kv, place = (int)blockIdx.x / c.n_head_kv, b = place / a.blocks;   // (heads lie side by side in a row)
     int lo, hi, len;
     kv4_seq(c, b, lo, hi, len);
     const int start = len - (hi - lo);
-    const int blk = (start >= 0 ? start / 32 : -((31 - start) / 32)) + (int)blockIdx.x % a.blocks;   // rows before position 0 are written too (as zeros)
+    const int blk = (start >= 0 ? start / 32 : -((31 - start) / 32)) + place % a.blocks;   // rows before position 0 are written too (as zeros)
     if (blk * 32 >= len || hi == lo) return;
     const uint8_t* src = kv4_block(c, b, h, blk);
     const int t_lo = start > blk * 32 ? start - blk * 32 : 0, t_hi = len - blk * 32 < 32 ? len - blk * 32 : 32;

@@ -67,9 +67,9 @@ static bool append_grid(Kv4Append& a, int max_rows, dim3& grid, const char*& err
     const Kv4Cache& c = a.c;
     if (max_rows > c.total) max_rows = c.total;
     a.blocks = (int)(((long long)max_rows + 62) / 32);
-    const long long x = (long long)a.blocks * c.n_seq;
+    const long long x = (long long)a.blocks * c.n_seq * c.n_head_kv;
     if (x > 0x7FFFFFFF) { err = "too many rows times sequences for one call"; return false; }
-    grid = dim3((unsigned)x, (unsigned)c.n_head_kv);
+    grid = dim3((unsigned)x);
     rows_vec(a.k);
     rows_vec(a.v);
     return true;

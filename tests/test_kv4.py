@@ -269,6 +269,12 @@ def test_a_nan_reaches_the_rows_that_see_it_and_no_others(dev):
     assert out.nonzero().tolist() == [[1, 0], [2, 1]]
 
 
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0])
+def test_scales_of_any_sign(dev, scale):
+    check_attention(dev, [45], [1], 4, 2, 64, 32, F16, scale=scale)
+    check_attention(dev, [140], [98], 4, 2, 32, 32, BF16, scale=scale)
+
+
 # ---- rows in and out ----------------------------------------------------------------------------------------------------------------------------
 def rows_like(shape, seed, dtype):
     x = torch.randn(shape, generator=torch.Generator().manual_seed(seed))
@@ -681,3 +687,110 @@ def test_c_interface(hip_lib):
         assert lib.ctamd_kv_compact(ops.TABLES.pack(4096, 0, 12288, 32768, 0, 20480, 1, 2, 3, 1), 16, 1, 48, 16, None, None, None) == -1
     finally:
         ops._lib = None
+
+
+# ---- more sequences than a wave has lanes, large pools, graphs, streams ----------------------------------------------------------------------------
+def test_more_sequences_than_lanes_share_the_line(dev):
+    """70 sequences, some without rows or tokens, in a table wide enough that the work is divided"""
+    rng = np.random.default_rng(3)
+    lens = [int(x) for x in rng.integers(0, 70, 70)]
+    lens[65] = 300
+    news = [int(min(x, n)) if n else int(x == 1) for x, n in zip(rng.integers(0, 3, 70), lens)]
+    check_attention(dev, lens, news, 2, 1, 32, 32, F16, seed=9, width=12)
+
+
+@pytest.mark.gpu
+def test_pages_beyond_4_gib(hip_lib):
+    """a pool of 5 GB: rows stored, read, attended to and copied in its last pages equal those in a small pool"""
+    ops.load(hip_lib)
+    dev = torch.device("cuda:0")
+    width = ops.kv4_page_bytes(8, 128, 256)
+    n_pages = 5 * 2**30 // width
+    big, small = torch.zeros((n_pages, width), dtype=torch.uint8, device=dev), torch.zeros((4, width), dtype=torch.uint8, device=dev)
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    k, v = (torch.randn((500, 8, 128), device=dev).half() for _ in range(2))
+    q = torch.randn((500, 16, 128), device=dev).half()
+    outs = []
+    for pages, table in ((big, i([n_pages - 1, n_pages - 3])), (small, i([1, 0]))):
+        ops.kv4_append(k, v, pages, table, i(500), None, 500, page_tokens=256)
+        rows = ops.kv4_read(pages, table, i(500), None, 500, 500, n_head_kv=8, head_dim=128, page_tokens=256)
+        one = ops.kv4_attention(q[-1:], pages, table, i(500), None, 1, n_head_kv=8, page_tokens=256)
+        outs.append(rows + (ops.kv4_attention(q, pages, table, i(500), None, 500, n_head_kv=8, page_tokens=256), one))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    # the partly filled last page is shared: making room copies it, from the pool's end to its start
+    refs = torch.zeros(n_pages, dtype=torch.int32, device=dev)
+    refs[n_pages - 1], refs[n_pages - 3] = 1, 2
+    t, n, r, short = ops.kv_reserve(big, i([n_pages - 1, n_pages - 3]), i(500), refs, i(3), page_tokens=256)
+    assert int(short) == 0 and t.tolist() == [[n_pages - 1, 0]] and torch.equal(big[0], big[n_pages - 3])
+    used = ops.kv_compact(big, t, r)
+    assert int(used[2]) == 3 and used[0].tolist() == [[2, 0]] and torch.equal(big[1], big[0])   # pages n - 3 and n - 1 go to the holes 1 and 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("news,width", [(1, 2), (1, 40), (70, 8)])
+def test_captured_and_replayed(hip_lib, news, width):
+    """append, attention, fork and room in one graph, two graphs at once, on a stream of their own: every replay equals the eager run on its inputs"""
+    ops.load(hip_lib)
+    dev = torch.device("cuda:0")
+    heads, H, dim, page, B = 2, 8, 64, 32, 3
+    n_pages = B * width + 4
+
+    def state(seed):
+        g = torch.Generator().manual_seed(seed)
+        table = torch.randperm(n_pages, generator=g)[:B * width].view(B, width).int().to(dev)
+        lens = torch.randint(news, width * page - 10, (B,), generator=g).int().clamp(min=news).to(dev)
+        refs = torch.zeros(n_pages, dtype=torch.int32)
+        refs[table.cpu().flatten().long()] = 1
+        x = [torch.randn((B * news, h, dim), generator=g).half().to(dev) for h in (H, heads, heads)]
+        return [torch.randint(0, 2, (n_pages, ops.kv4_page_bytes(heads, dim, page)), generator=g, dtype=torch.uint8).to(dev), table, lens, refs.to(dev),
+                torch.randint(-1, B, (B,), generator=g).int().to(dev)] + x
+
+    cu = (torch.arange(B + 1) * news).int().to(dev)
+
+    def run(pages, table, lens, refs, parents, q, k, v):
+        ops.kv4_append(k, v, pages, table, lens, cu, news, page_tokens=page)
+        out = ops.kv4_attention(q, pages, table, lens, cu, news, n_head_kv=heads, page_tokens=page)
+        t, n, r = ops.kv_fork(table, lens, refs, parents, page_tokens=page)
+        t, n, r, short = ops.kv_reserve(pages, t, n, r, torch.ones_like(n), page_tokens=page)
+        return [out, t, n, r, short, pages]
+
+    stream = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        s = state(0)
+        with torch.cuda.stream(stream):
+            run(*[x.clone() for x in s])
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs = run(*s)
+        graphs.append((graph, s, outs, torch.cuda.Stream()))
+    for seed in range(1, 7):
+        wants = []
+        for k, (graph, s, outs, _) in enumerate(graphs):
+            new = state(10 * seed + k)
+            for x, y in zip(s, new):
+                x.copy_(y)
+            wants.append([x.clone() for x in run(*new)])
+        torch.cuda.synchronize()
+        for graph, s, outs, mine in graphs:
+            with torch.cuda.stream(mine):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (graph, s, outs, _), want in zip(graphs, wants):
+            assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+@pytest.mark.gpu
+def test_same_bits_every_time(hip_lib):
+    ops.load(hip_lib)
+    dev = torch.device("cuda:0")
+    for news, width in ((1, 60), (40, 30)):
+        c = Cache(4, [900, 30, 511], 2, 64, 32, extra_width=width)
+        c.fill(5)
+        pages, table, n = c.on(dev)
+        q = torch.randn((3 * news, 16, 64), device=dev).half()
+        cu = torch.tensor([0, news, 2 * news, 3 * news], dtype=torch.int32, device=dev)
+        first = ops.kv4_attention(q, pages, table, n, cu, news, n_head_kv=2, page_tokens=32)
+        for _ in range(5):
+            assert torch.equal(first, ops.kv4_attention(q, pages, table, n, cu, news, n_head_kv=2, page_tokens=32))
