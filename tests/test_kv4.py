@@ -5,7 +5,13 @@ Tolerances, from the roundings that the kernels make (ops.kv4_attention): p and 
 v with weights p, so an element is off by at most (2^-11 + 2^-11) A with A = sum p |v| / sum p.  An error of e in a score (natural units) changes every weight by a
 factor within exp(+-e): 2 e A.  A score's error: f32 sums, (D + 8) 2^-24 scale sum |q| |k|; the exponent's argument, (4 |s| + 8) 2^-23; queries that are not
 halves already, 2^-11 scale sum |q| |k| (float32) or the part below f16's range after the row's power of two, 2^-25 max |q| scale sum |k| (bf16); and in the
-many-row kernel K's values as halves, 2^-11 scale sum |q| |k|.  The result's own rounding is half a step of its type."""
+many-row kernel K's values as halves, 2^-11 scale sum |q| |k|.  The result's own rounding is half a step of its type.
+
+Halves below 2^-14 are multiples of 2^-24, so there a rounding is off by up to 2^-25 absolutely.  That happens to p (the largest weight is at least 1: weights are
+relative to a running maximum, which no final maximum is below), 2^-25 sum |v| / sum p <= 2^-25 sum |v| in the result; in the few-row kernel the second half of p has
+the same spacing, so it does not help there.  And it happens to float16 results, 2^-25.  (V's values are exempt: d is a multiple of 2^-24 and so is d (code - 8).)
+attention64 adds both to A, divided by the 2^-10 that A is multiplied with.  A row whose largest weight belongs to a value of 0 shows it: A is then 1e-9 of its
+neighbours' values, and the bound without these terms is smaller than the spacing of the type that the result has."""
 import math
 import os
 import re
@@ -136,7 +142,7 @@ def attention64(q, values, heads_kv, scale, extra):
             s = kk @ q[i, h] * scale
             p = np.exp(s - s.max())
             p /= p.sum()
-            out[i, h], mag[i, h] = p @ vv, p @ np.abs(vv)
+            out[i, h], mag[i, h] = p @ vv, p @ np.abs(vv) + 2.0**-15 * np.abs(vv).sum(0) + 2.0**-15
             dots = (np.abs(kk) @ np.abs(q[i, h])).max() * abs(scale)
             err[i, h] = ((D + 8) * 2.0**-24 + extra[0]) * dots + extra[1] * np.abs(q[i, h]).max() * np.abs(kk).sum(-1).max() * abs(scale) + (4 * np.abs(s).max() + 8) * 2.0**-23
     return out, mag, err
