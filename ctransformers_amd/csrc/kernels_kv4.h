@@ -212,7 +212,8 @@ DEV const uint8_t* kv4_in_page(const Kv4Cache& c, int pid, int h, int blk) {
 // One workgroup per (block, head) that new rows fall into: it alone writes that block, so a V dword that keeps older tokens is read, changed and written without
 // atomics.  A lane takes eight dims (16 bytes of a half row, so that a wave reads whole lines), four lanes a group; they agree on the largest value by two quad
 // exchanges.  K codes and scales go straight out, V codes cross the workgroup through LDS (eight tokens to a dword).  All loads of a lane are issued before the
-// first value is used.
+// first value is used.  16 prompts of up to 1500 tokens, 64 heads of 112 in float32 (585 MB in, 101 MB out): 217 us, 3.2 TB/s; one token of 64 sequences, 8 heads:
+// 6.4 us, latency (cursor -> table -> rows -> codes -> store).
 template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
     __shared__ uint32_t vcode[32][8 * G + 1];   // V codes as bytes [token][dim]; + 1: tokens in different banks
     __shared__ uint16_t sc[2][32][G];
@@ -318,6 +319,7 @@ template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const 
 }
 
 // The last rows of every sequence out of the cache, as numbers: the mirror image of kv4_append_kernel, same workgroups.  Rows whose page is absent are zeros.
+// The same prompts (101 MB in, 292 MB of halves out): 119 us, 3.3 TB/s.
 template <int G> __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Append a) {
     const Kv4Cache& c = a.c;
     const int tid = (int)threadIdx.x, h = (int)blockIdx.x % c.n_head_kv, place = (int)blockIdx.x / c.n_head_kv, b = place / a.blocks;   // (heads lie side by side in a row)
@@ -465,6 +467,8 @@ DEV u32x4 kv4_values(uint32_t w, uint32_t s0, uint32_t s1, uint32_t s2, uint32_t
 // multiplies the 32-dim product in f32, so K is used exactly.  Maximum, sum and O stay per lane in f32; the maximum is raised (and O rescaled) only when a score
 // passes it by more than 2^8, so most blocks exchange nothing between lanes (p <= 256 fits f16 as well as p <= 1 does).  P enters as two halves, the rounded one and
 // what it left (the matrix cores have the time: +2 % at most), so that what is rounded on the way is V's product with its scale alone.
+// Memory-bound: one sequence of 130 000 tokens, 8 KV heads of 128 with 8 query heads each (150 MB): 34 us, 4.4 TB/s; 64 sequences of 0 .. 8192 tokens (306 MB): 70 us,
+// 4.4 TB/s (a large copy moves 4.66).  One sequence of 140 tokens: 7.2 us, latency.
 // The next block's K is fetched into the registers of this one's as soon as its scores are there, its V after the V product: 40 dwords a lane at 128 dims for a
 // block in flight, which leaves room for four waves a SIMD.
 template <int G> DEV void kv4_fetch_k(uint32_t (&kc)[2][G], uint32_t (&ks)[2][2 * G], const uint8_t* blk, int m, int i) {
@@ -716,7 +720,8 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
 }
 
 // The parts of a row joined: a workgroup of W waves per (row, head); a wave takes every W-th part, four at a time, two dims a lane, with a maximum of its own.
-// LINE: parts are shares' ends (kv4_decode_kernel), else the splits of kv4_prompt_kernel.
+// LINE: parts are shares' ends (kv4_decode_kernel), else the splits of kv4_prompt_kernel.  6.5 us for 64 rows of 95 parts as for 4096 rows of one or two: latency.
+// (A join by the last workgroup to arrive would save this launch, but its counters would have to survive between calls: two graphs could meet in them.)
 template <int NR, bool LINE, int W> __global__ void __launch_bounds__(64 * W) kv4_join_kernel(const Kv4Attn a, int tile_rows) {
     __shared__ float acc[W][128 * NR], stat[W][2];
     const Kv4Cache& c = a.c;
@@ -808,6 +813,12 @@ template <int NR, bool LINE, int W> __global__ void __launch_bounds__(64 * W) kv
 // V as 16-byte chunks [4 eights of tokens][dim]: both are read and written without bank conflicts.  Two buffers: while one pair of blocks is computed the next is
 // fetched into registers, unpacked and written into the other, one barrier a pair.
 // The row tiles of one (sequence, KV head) go to one XCD, whose L2 then holds that head's codes for all of them; tiles that see most come first.
+// Rounded on the way: K's and V's values and p to halves (2^-11 each at most; the 32 x 32 products want halves).  A float16 result is off by 3.8e-4 of its norm, its own
+// rounding alone by 2.1e-4; K exact, as in the kernel above, would take 128 more fused multiply-adds and 32 more LDS reads a step.
+// 2048 tokens, 32 heads of 128 (34 GFLOP): 79 us, 437 TFLOP/s; 4 chunks of up to 512 behind up to 8000 tokens, 64 / 8 heads (234 GFLOP): 372 us, 630 TFLOP/s (a large
+// f16 product: 1142).  Bound by the vector units: 270 instructions a step and wave (exp2 a quarter of their time) take 1300 cycles beside 1024 of matrix products, two
+// waves a SIMD overlap them in part; 33 % of the waves' time is waits.  Measured and not taken: one block a step and three waves a SIMD (96 / 421 us), unpacking
+// between the K.Q products (82 / 371), wave priorities around them (no change), all pairs' long tiles first (chunks 635).
 template <int G> struct Kv4Lds { static constexpr int KC = 32 * 16 + 32, KB = 4 * G * KC, VB = 4 * 32 * G * 16, BLK = KB + VB, BYTES = 4 * BLK; };
 
 #ifdef CT_EMU
