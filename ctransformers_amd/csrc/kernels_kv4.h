@@ -520,7 +520,7 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
         b = uniform_int((int)blockIdx.x / per_seq);
         in_seq = (int)blockIdx.x - b * per_seq;
     }
-  while (x < x_end) {
+  while (x < x_end && b < c.n_seq) {   // (the second holds by itself unless lens or cu change meanwhile)
     const int lane = kv4_anew(lane_id()), m = lane & 15, i = lane >> 4;
     int lo, hi, len;
     kv4_seq(c, b, lo, hi, len);
