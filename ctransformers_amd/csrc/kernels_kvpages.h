@@ -112,14 +112,15 @@ __global__ void __launch_bounds__(kPlanThreads) kv_reserve_plan_kernel(const KvP
     int taken = 0, copies = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += kPlanThreads) {
         const int s = s0 + tid;
-        int need = 0, start = 0, tail = -1, len = 0, more = 0, first = 0, last = 0;
+        int need = 0, start = 0, tail = -1, len = 0, more = 0, first = 0;
+        long long last = 0;                          // (a sequence may end near 2^31, and a page be one token)
         bool partly = false;
         if (s < a.n_seq) {
             len = kvp_len(a, s);
             more = a.add[s] > 0 ? a.add[s] : 0;
             const long long to = (long long)len + more;
             first = len / a.page_tokens;
-            last = (int)((to + a.page_tokens - 1) / a.page_tokens);
+            last = (to + a.page_tokens - 1) / a.page_tokens;
             if (more && last > a.width) flags = 1;   // (several threads may write it: the same value)
             partly = more && len % a.page_tokens != 0;
             if (partly && first < a.width) {
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_reserve_plan_kernel(const KvP
         }
         if (more) {
             start = first + (partly && tail >= 0 && !copied);
-            need = last - start < a.width ? last - start : a.width;   // (more than that is refused below)
+            need = last - start < a.width ? (int)(last - start) : a.width;   // (more than that is refused below)
         }
         __syncthreads();                             // every thread has read the earlier rounds' tails
         int all, c_all;
