@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_reserve_plan_kernel(const KvP
             const long long to = (long long)len + more;
             first = len / a.page_tokens;
             last = (to + a.page_tokens - 1) / a.page_tokens;
-            if (more && last > a.width) flags = 1;   // (several threads may write it: the same value)
+            if (more && (last > a.width || to > 0x7FFFFFFF)) flags = 1;   // (several threads may write it: the same value)
             partly = more && len % a.page_tokens != 0;
             if (partly && first < a.width) {
                 const int p = a.table[(long long)s * a.width + first];

@@ -265,7 +265,7 @@ def kv_fork(table, lens, refs, parents, *, page_tokens, keep=None):
 def kv_reserve(pages, table, lens, refs, add, *, page_tokens):
     """(table, lens, refs, short) with room for add[i] more tokens in sequence i: lens grows by it, pages are taken lowest free first in the order of the sequences,
     and a last page that others share is copied before its sequence writes it.  pages: [n_pages, ..] or [layers, n_pages, ..], any type.  short (int32, on the
-    device): 0, or the pages that were missing, or -1 where a sequence outgrows its row of the table; then nothing has changed."""
+    device): 0, or the pages that were missing, or -1 where a sequence outgrows its row of the table, or 2^31 - 1 tokens; then nothing has changed."""
     device = _device_of("table", table)
     _ints(device, "refs", refs, 1)
     n_seq = table.shape[0]

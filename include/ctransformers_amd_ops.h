@@ -64,7 +64,7 @@ typedef struct {
 int ctamd_kv_fork(const ctamd_kv_tables* t, const int* parents, const int* keep, int n_new, void* stream);
 /* Room for add[s] more tokens: lens_out = lens + add, the pages for them taken lowest free first in the order of the sequences, and a shared last page that will be
  * written is copied (pages [layers] x layer_stride bytes of n_pages pages of page_bytes, a multiple of 16).  *status: 0; or the pages that were missing, or -1 where a
- * sequence would outgrow the table — then nothing changes.  ws: ctamd_kv_reserve_ws() ints. */
+ * sequence would outgrow the table, or 2^31 - 1 tokens — then nothing changes.  ws: ctamd_kv_reserve_ws() ints. */
 long long ctamd_kv_reserve_ws(int n_seq, int n_pages);
 int ctamd_kv_reserve(const ctamd_kv_tables* t, const int* add, void* pages, int layers, long long layer_stride, long long page_bytes, int* status, int* ws,
                      void* stream);
