@@ -572,7 +572,7 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
 
     uint32_t kc[2][G], ks[2][2 * G], vc[2 * G], vs[2 * G + 2 * (G & 1)];
     int blk = begin + w;
-    if (c.n_pages <= 0) end = begin;
+    if (c.n_pages <= 0 || c.table_width <= 0) end = begin;   // (nothing to see: the unit's one block is not looked up)
     // Loads are never conditional (a wait for V would have to count K's as not issued, and wait for them too): where there is no block, the pool's first is read
     // and everything in it masked.
     bool here = false;

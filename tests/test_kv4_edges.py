@@ -3,11 +3,38 @@ import pytest
 import torch
 
 from ctransformers_amd import ops
-from test_kv4 import dev  # noqa: F401  (the fixture)
+from test_kv4 import Cache, dev  # noqa: F401  (the fixture)
 
 
 def ints(dev, *x):
     return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def c_attention(dev, q, pages, table, lens, cu, rows, heads_kv, page, out, width, stride):
+    """ctamd_kv4_attention with a table of `width` entries that lie where `table` begins, and what it returns"""
+    total, H, dim = q.shape
+    types = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+    c = ops.CACHE.pack(pages.data_ptr(), table.data_ptr(), lens.data_ptr(), cu.data_ptr(), pages.stride(0), pages.shape[0], stride, width, lens.shape[0], total, heads_kv, dim, page, rows)
+    row = lambda x: ops.ROWS.pack(x.data_ptr(), *x.stride(), types[x.dtype])  # noqa: E731
+    n = ops._lib.ctamd_kv4_attention_ws(c, H)
+    ws = torch.empty(max(n, 1), dtype=torch.float32, device=dev)
+    code = ops._lib.ctamd_kv4_attention(c, H, row(q), row(out), dim**-0.5, ws.data_ptr(), n, ops._stream(dev.index) if dev.type == "cuda" else None)
+    if dev.type == "cuda":
+        torch.cuda.synchronize()
+    return code
+
+
+# ---- attention ------------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("news", [1, 20, 100])
+def test_a_table_without_entries(dev, news):
+    """the memory behind it names a page: it is no entry of the table, and no row sees anything"""
+    c = Cache(1, [40], 1, 64, 32, extra_width=3)
+    c.fill(2)
+    pages, table, lens = c.on(dev)
+    q = torch.ones((news, 2, 64), dtype=torch.float16, device=dev)
+    out = torch.full_like(q, 7)
+    assert c_attention(dev, q, pages, table, lens, ints(dev, 0, news), news, 1, 32, out, 0, 4) == 0
+    assert (out == 0).all()
 
 
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
