@@ -49,7 +49,7 @@ bool kv4_check(Kv4Cache& c, int page_tokens, const char*& err) {
     else if (c.n_seq < 0 || c.total < 0 || c.n_pages < 0 || c.table_width < 0 || c.table_stride < c.table_width) err = "negative size, or table rows that overlap";
     else if (c.n_seq > (1 << 20) || c.total > (1 << 24)) err = "at most 2^20 sequences and 2^24 rows a call";
     else if ((long long)c.table_width * page_tokens > (1 << 30)) err = "table rows of more than 2^30 tokens";
-    else if (c.n_seq && c.total && (!c.table || !c.lens || !c.pages) && c.n_pages) err = "null cache pointer";
+    else if (c.n_seq && c.total && ((!c.table && c.table_width) || !c.lens || !c.pages) && c.n_pages) err = "null cache pointer";
     else if (c.n_seq != 1 && !c.cu && c.total) err = "cu is needed for more than one sequence";
     else if (c.page_stride < bytes && c.n_pages > 1) err = "pages overlap: page_stride is less than a page";
     else if (c.page_stride % 16 || (uintptr_t)c.pages % 16) err = "pages are 16-byte aligned";

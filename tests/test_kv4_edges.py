@@ -37,6 +37,20 @@ def test_a_table_without_entries(dev, news):
     assert (out == 0).all()
 
 
+@pytest.mark.parametrize("n_pages", [0, 3])
+def test_sequences_that_have_no_pages_yet(dev, n_pages):
+    """a table of no columns is an empty tensor, whose address is null: rows are not stored, read back as zeros and see nothing"""
+    pages = torch.full((n_pages, ops.kv4_page_bytes(2, 64, 32)), 5, dtype=torch.uint8, device=dev)
+    table, lens, cu = torch.empty((2, 0), dtype=torch.int32, device=dev), ints(dev, 0, 3), ints(dev, 0, 0, 3)
+    x = torch.ones((3, 2, 64), dtype=torch.float16, device=dev)
+    old = pages.clone()
+    ops.kv4_append(x, x, pages, table, lens, cu, 3, page_tokens=32)
+    assert torch.equal(pages, old)
+    for rows in ops.kv4_read(pages, table, lens, cu, 3, 3, n_head_kv=2, head_dim=64, page_tokens=32):
+        assert (rows == 0).all()
+    assert (ops.kv4_attention(x, pages, table, lens, cu, 3, n_head_kv=2, page_tokens=32) == 0).all()
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("length,add", [(2**31 - 1, 2**31 - 1), (1, 2**31 - 1), (2**31 - 1, 1), (2**30, 2**30)])
 def test_room_behind_lengths_near_2_31(dev, length, add):
