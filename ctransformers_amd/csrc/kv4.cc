@@ -75,6 +75,13 @@ static bool append_grid(Kv4Append& a, int max_rows, dim3& grid, const char*& err
     return true;
 }
 
+// A pool of no pages: nothing is stored, but reading and attention look at the lengths and the table all the same.
+static bool tables_there(const Kv4Cache& c, const char*& err) {
+    if (c.lens && (c.table || !c.table_width)) return true;
+    err = "null cache pointer";
+    return false;
+}
+
 bool kv4_append(Kv4Append& a, int max_rows, hipStream_t stream, const char*& err) {
     dim3 grid;
     if (a.c.total == 0 || a.c.n_seq == 0 || a.c.n_pages == 0 || max_rows <= 0) return true;
@@ -86,7 +93,7 @@ bool kv4_append(Kv4Append& a, int max_rows, hipStream_t stream, const char*& err
 bool kv4_read(Kv4Append& a, int max_rows, hipStream_t stream, const char*& err) {
     dim3 grid;
     if (a.c.total == 0 || a.c.n_seq == 0 || max_rows <= 0) return true;
-    if (!append_grid(a, max_rows, grid, err)) return false;
+    if (!tables_there(a.c, err) || !append_grid(a, max_rows, grid, err)) return false;
     KV4_BY_GROUPS(a.c.groups, CT_LAUNCH(kv4_read_kernel<G>, grid, dim3(256), stream, a);)
     return launched(err);
 }
@@ -167,6 +174,7 @@ bool kv4_attention(Kv4Attn& a, int max_rows, long long ws_floats, hipStream_t st
     if (a.n_head < 1 || a.n_head > 65536 || a.n_head % c.n_head_kv) { err = "n_head is a multiple of n_head_kv"; return false; }
     if (a.q.dim != 1) { err = "the dims of a query row are adjacent"; return false; }
     if (c.total == 0 || c.n_seq == 0 || max_rows <= 0) return true;
+    if (!tables_there(c, err)) return false;
     const long long want = kv4_attention_plan(a, max_rows);
     if (want > ws_floats || (want && !a.ws)) { err = "workspace too small"; return false; }
     const long long pairs = (long long)c.n_seq * c.n_head_kv, grid = ((pairs + 7) & ~7ll) * a.tiles * a.nsplit;

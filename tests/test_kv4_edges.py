@@ -51,6 +51,17 @@ def test_sequences_that_have_no_pages_yet(dev, n_pages):
     assert (ops.kv4_attention(x, pages, table, lens, cu, 3, n_head_kv=2, page_tokens=32) == 0).all()
 
 
+def test_a_pool_of_no_pages_still_needs_lengths(dev):
+    """the C interface: no page is touched, but the sequences' lengths are read all the same; null ones are an error, not an access"""
+    x = torch.ones((1, 2, 64), dtype=torch.float16, device=dev)
+    row, table = ops.ROWS.pack(x.data_ptr(), *x.stride(), 0), ints(dev, 0)
+    for t, lens in ((table.data_ptr(), 0), (0, table.data_ptr())):
+        c = ops.CACHE.pack(0, t, lens, 0, 36864, 0, 1, 1, 1, 1, 2, 64, 32, 1)
+        assert ops._lib.ctamd_kv4_read(c, row, row, None) == -1 and b"null cache pointer" in ops._lib.ctamd_ops_error()
+        assert ops._lib.ctamd_kv4_attention(c, 2, row, row, 1.0, None, 0, None) == -1 and b"null cache pointer" in ops._lib.ctamd_ops_error()
+        assert ops._lib.ctamd_kv4_append(c, row, row, None) == 0   # (nothing to do)
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("length,add", [(2**31 - 1, 2**31 - 1), (1, 2**31 - 1), (2**31 - 1, 1), (2**30, 2**30)])
 def test_room_behind_lengths_near_2_31(dev, length, add):
