@@ -735,6 +735,7 @@ template <int NR, bool LINE, int W> __global__ void __launch_bounds__(64 * W) kv
     }
     int lo, hi, len;
     kv4_seq(c, b, lo, hi, len);
+    if (row < lo) return;   // (cu does not ascend)
     const int kvh = head / a.rep, r = (row - lo) * a.rep + head % a.rep, tile = r / tile_rows, dim = c.head_dim;
     const long long step = (long long)tile_rows * (dim + 2);
     int parts;

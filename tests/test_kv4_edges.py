@@ -62,6 +62,17 @@ def test_a_pool_of_no_pages_still_needs_lengths(dev):
         assert ops._lib.ctamd_kv4_append(c, row, row, None) == 0   # (nothing to do)
 
 
+def test_rows_between_sequences_are_left_as_they_are(dev):
+    """cu that does not ascend (whose own rows are undefined): a row that no sequence holds is not joined from memory in front of another row's parts"""
+    c = Cache(1, [600, 40, 600], 1, 32, 32, extra_width=8)
+    c.fill(2)
+    pages, table, lens = c.on(dev)
+    q = torch.ones((9, 2, 32), dtype=torch.float16, device=dev)
+    out = torch.full_like(q, 7)
+    ops.kv4_attention(q, pages, table, lens, ints(dev, 7, 9, 2, 3), 2, n_head_kv=1, page_tokens=32, out=out)
+    assert (out[[0, 1, 3, 4, 5, 6]] == 7).all()
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("length,add", [(2**31 - 1, 2**31 - 1), (1, 2**31 - 1), (2**31 - 1, 1), (2**30, 2**30)])
 def test_room_behind_lengths_near_2_31(dev, length, add):
