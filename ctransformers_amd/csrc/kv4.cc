@@ -3,6 +3,7 @@
 #include "kernels_kv4.h"
 #include "kernels_kvpages.h"
 
+#include <float.h>
 #include <stdio.h>
 #include <string.h>
 
@@ -172,6 +173,7 @@ template <int W> static void launch_join(const Kv4Attn& a, int tr, dim3 grid, hi
 bool kv4_attention(Kv4Attn& a, int max_rows, long long ws_floats, hipStream_t stream, const char*& err) {
     const Kv4Cache& c = a.c;
     if (a.n_head < 1 || a.n_head > 65536 || a.n_head % c.n_head_kv) { err = "n_head is a multiple of n_head_kv"; return false; }
+    if (!(a.scale >= -FLT_MAX && a.scale <= FLT_MAX)) { err = "scale is not a finite number"; return false; }
     if (a.q.dim != 1) { err = "the dims of a query row are adjacent"; return false; }
     if (c.total == 0 || c.n_seq == 0 || max_rows <= 0) return true;
     if (!tables_there(c, err)) return false;

@@ -73,6 +73,20 @@ def test_rows_between_sequences_are_left_as_they_are(dev):
     assert (out[[0, 1, 3, 4, 5, 6]] == 7).all()
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 1e39])
+def test_scales_that_are_no_numbers(dev, scale):
+    """refused (a NaN used to give the mean of V); 1e39 is infinite as the float that it is passed as"""
+    c = Cache(1, [40], 1, 32, 32)
+    c.fill(2)
+    pages, table, lens = c.on(dev)
+    for news in (1, 40, 200):
+        q = torch.ones((news, 1, 32), dtype=torch.float16, device=dev)
+        out = torch.full_like(q, 7)
+        with pytest.raises(ValueError, match="scale"):
+            ops.kv4_attention(q, pages, table, lens, None, news, n_head_kv=1, page_tokens=32, scale=scale, out=out)
+        assert (out == 7).all()
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("length,add", [(2**31 - 1, 2**31 - 1), (1, 2**31 - 1), (2**31 - 1, 1), (2**30, 2**30)])
 def test_room_behind_lengths_near_2_31(dev, length, add):
