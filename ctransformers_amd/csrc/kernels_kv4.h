@@ -143,9 +143,18 @@ template <int N, class Across> DEV float kv4_query(u32x4 (&q)[N], const Kv4Rows&
         for (int j = 0; j < 8; ++j) { x[k][j] = in ? x[k][j] : 0.0f; big = fmaxf(big, fabsf(x[k][j])); }
     }
     big = across(big);
-    float up = 1.0f, down = 1.0f;
-    const int e = (int)((bits_of(big) >> 23) & 255u);
-    if (e > 0 && e < 254) { up = float_of((uint32_t)(254 - e) << 23); down = float_of((uint32_t)e << 23); }
+    float up = 1.0f, down = 1.0f, low = 1.0f;
+    if (big < 0x1p-64f && big > 0.0f) {   // subnormals' exponents say nothing: 2^64 more, exactly
+        big *= 0x1p64f;
+        low = 0x1p-64f;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[k][j] *= 0x1p64f;
+    }
+    int e = (int)((bits_of(big) >> 23) & 255u);
+    e = e == 254 ? 253 : e;               // (the largest rows come to [2, 4): 2^-127 is no normal number)
+    if (e > 0 && e < 254) { up = float_of((uint32_t)(254 - e) << 23); down = float_of((uint32_t)e << 23) * low; }
 #pragma unroll
     for (int k = 0; k < N; ++k)
         q[k] = u32x4_of(kv4_cvt2(x[k][0] * up, x[k][1] * up) ^ flip, kv4_cvt2(x[k][2] * up, x[k][3] * up) ^ flip, kv4_cvt2(x[k][4] * up, x[k][5] * up) ^ flip,
@@ -153,7 +162,7 @@ template <int N, class Across> DEV float kv4_query(u32x4 (&q)[N], const Kv4Rows&
     return down;
 }
 // the factor of a score in front of exp2: positive, also for a scale of 0 (whose scores are then as good as equal), so that -inf stays what it is
-DEV float kv4_factor(float scale, float down, float unit) { return fmaxf(fabsf(scale) * 1.44269504088896f * down * unit, 1e-30f); }
+DEV float kv4_factor(float scale, float down, float unit) { return fmaxf((fabsf(scale) * down) * (1.44269504088896f * unit), 1e-30f); }   // (neither factor overflows before the other has scaled it)
 // eight neighbouring dims out; vec: as for loads
 DEV void kv4_store8(void* p, long long at, int type, int vec, const float (&x)[8]) {
     if (vec && type != KV4_F32) {

@@ -1,9 +1,10 @@
 """The 4-bit paged KV cache (ctransformers_amd/ops.py, csrc/engine_kv4.h) at the edges of what its calls accept."""
+import numpy as np
 import pytest
 import torch
 
 from ctransformers_amd import ops
-from test_kv4 import Cache, dev  # noqa: F401  (the fixture)
+from test_kv4 import Cache, attention64, dev  # noqa: F401  (the fixture)
 
 
 def ints(dev, *x):
@@ -85,6 +86,30 @@ def test_scales_that_are_no_numbers(dev, scale):
         with pytest.raises(ValueError, match="scale"):
             ops.kv4_attention(q, pages, table, lens, None, news, n_head_kv=1, page_tokens=32, scale=scale, out=out)
         assert (out == 7).all()
+
+
+def far_rows(dev, news, big, scale, dtype, k_scale):
+    """rows of magnitude `big` (times 1 .. 4), keys of k_scale: kv4_attention against the 64-bit formula, with the bound that test_kv4.py derives; the queries are exact
+    as halves (few bits), but bf16's and float32's roundings to halves are allowed for all the same"""
+    c = Cache(1, [40 + news], 1, 64, 32)
+    c.fill(2, k_scale)
+    q = (torch.randint(-3, 4, (news, 2, 64), generator=torch.Generator().manual_seed(4)).double() * big).to(dtype)
+    assert q.isfinite().all() and (q.double().abs().max() >= 2 * big)
+    pages, table, n = c.on(dev)
+    got = ops.kv4_attention(q.to(dev), pages, table, n, None, news, n_head_kv=1, page_tokens=32, scale=scale, out=torch.empty(q.shape, dtype=torch.float32, device=dev)).double().cpu().numpy()
+    want, mag, err = attention64(q.double().numpy(), c.values[0], 1, float(np.float32(scale)), (2.0**-11, 2.0**-25))
+    assert err.max() < 0.1   # (the bound says something)
+    assert (np.abs(got - want) <= mag * (2.0**-10 + 2 * np.expm1(err)[..., None]) * 1.01 + np.abs(want) * 2.0**-24 * 1.01).all()
+
+
+@pytest.mark.parametrize("news", [1, 20, 100])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_queries_at_the_ends_of_their_type(dev, dtype, news):
+    """the largest values (beyond 2^127) with a small scale, subnormal ones with a large scale and large keys"""
+    far_rows(dev, news, 2.0**126, 2.0**-129, dtype, 1.0)
+    far_rows(dev, news, 2.0**-133, 2.0**120, dtype, 1024.0)
+    if dtype == torch.float32:
+        far_rows(dev, news, 2.0**-147, 1.5 * 2.0**127, dtype, 8192.0)
 
 
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
