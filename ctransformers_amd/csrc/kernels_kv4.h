@@ -161,8 +161,12 @@ template <int N, class Across> DEV float kv4_query(u32x4 (&q)[N], const Kv4Rows&
                         kv4_cvt2(x[k][6] * up, x[k][7] * up) ^ flip);
     return down;
 }
-// the factor of a score in front of exp2: positive, also for a scale of 0 (whose scores are then as good as equal), so that -inf stays what it is
-DEV float kv4_factor(float scale, float down, float unit) { return fmaxf((fabsf(scale) * down) * (1.44269504088896f * unit), 1e-30f); }   // (neither factor overflows before the other has scaled it)
+// The factor of a score in front of exp2: positive, also for a scale of 0 (whose scores are then as good as equal), so that -inf stays what it is; and at most 2^100,
+// where unequal scores (2^-72 apart at least) have become as far apart as exp2 can tell, and none overflows (below 2^26).
+DEV float kv4_factor(float scale, float down, float unit) { return fminf(fmaxf((fabsf(scale) * down) * (1.44269504088896f * unit), 1e-30f), 0x1p100f); }
+// exp2's arguments are fma(score, factor, -maximum): one shift by the rounded maximum for all of a row's weights, which their quotients do not see.  From here on that
+// rounding could carry the largest weight out of the halves' range (and out of exp2's, further up): such rows round the products first, so that the maximum is one of them.
+constexpr float kFar = 0x1p22f;
 // eight neighbouring dims out; vec: as for loads
 DEV void kv4_store8(void* p, long long at, int type, int vec, const float (&x)[8]) {
     if (vec && type != KV4_F32) {
@@ -648,11 +652,17 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
 #pragma unroll
                         for (int e = 0; e < 4; ++e) O[n][j][e] *= f;
                 }
-                const float base = mx[n] == -INFINITY ? 0.0f : -mx[n];
+                float base = mx[n] == -INFINITY ? 0.0f : -mx[n], factor = sc2[n];
+                if (__ballot(fabsf(base) > kFar)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[n][e / 4][e & 3] = s[n][e / 4][e & 3] * factor + base;
+                    factor = 1.0f;
+                    base = 0.0f;
+                }
                 uint32_t pk[4], lo[4];
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const float x = exp2_fast(fmaf(s[n][p / 2][2 * (p & 1)], sc2[n], base)), y = exp2_fast(fmaf(s[n][p / 2][2 * (p & 1) + 1], sc2[n], base));
+                    const float x = exp2_fast(fmaf(s[n][p / 2][2 * (p & 1)], factor, base)), y = exp2_fast(fmaf(s[n][p / 2][2 * (p & 1) + 1], factor, base));
                     pk[p] = kv4_cvt2(x, y);
                     sum[n] += x;
                     sum[n] += y;
@@ -960,7 +970,13 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
 #pragma unroll
                 for (int e = 0; e < 16; ++e) O[g][e] *= f;
         }
-        const float base = mx == -INFINITY ? 0.0f : -mx;
+        float base = mx == -INFINITY ? 0.0f : -mx, factor = sc2;
+        if (__ballot(fabsf(base) > kFar)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) S[e / 16][e & 15] = S[e / 16][e & 15] * factor + base;
+            factor = 1.0f;
+            base = 0.0f;
+        }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const unsigned char* vb = smem + (buf * 2 + k) * L::BLK + L::KB;
@@ -969,7 +985,7 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
                 uint32_t pk[4];
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    const float x = exp2_fast(fmaf(S[k][8 * t + e], sc2, base)), y = exp2_fast(fmaf(S[k][8 * t + e + 1], sc2, base));
+                    const float x = exp2_fast(fmaf(S[k][8 * t + e], factor, base)), y = exp2_fast(fmaf(S[k][8 * t + e + 1], factor, base));
                     pk[e / 2] = kv4_cvt2(x, y);
                     sum = kv4_sum2(pk[e / 2], sum);
                 }
