@@ -167,6 +167,9 @@ DEV float kv4_factor(float scale, float down, float unit) { return fminf(fmaxf((
 // exp2's arguments are fma(score, factor, -maximum): one shift by the rounded maximum for all of a row's weights, which their quotients do not see.  From here on that
 // rounding could carry the largest weight out of the halves' range (and out of exp2's, further up): such rows round the products first, so that the maximum is one of them.
 constexpr float kFar = 0x1p22f;
+// Weights are halves for the matrix instructions.  They are relative to a number that lies kRaise below the row's running maximum and is moved only when a score passes that
+// maximum by more than kLag: at most 2^15, and what is lost at the small end lies 2^-(24 + kRaise) below the maximum instead of 2^-24 (a long flat tail counts).
+constexpr float kRaise = 11.0f, kLag = 15.0f - kRaise;   // (times of all sizes: the same with 7, 9 and 11; with 14 maxima move often, prompts take 5 % longer)
 // eight neighbouring dims out; vec: as for loads
 DEV void kv4_store8(void* p, long long at, int type, int vec, const float (&x)[8]) {
     if (vec && type != KV4_F32) {
@@ -478,8 +481,8 @@ DEV u32x4 kv4_values(uint32_t w, uint32_t s0, uint32_t s1, uint32_t s2, uint32_t
 //   O = V^T (A: lane = dim) x P (B: lane = row): those eight probabilities ARE the lane's k slots — V is stored in that order
 // K's codes enter as f16 SUBNORMALS, the 16-bit integers themselves (code * 2^-24: no conversion); -8 * sum(Q) is the product's C operand and the group's scale
 // multiplies the 32-dim product in f32, so K is used exactly.  Maximum, sum and O stay per lane in f32; the maximum is raised (and O rescaled) only when a score
-// passes it by more than 2^8, so most blocks exchange nothing between lanes (p <= 256 fits f16 as well as p <= 1 does).  P enters as two halves, the rounded one and
-// what it left (the matrix cores have the time: +2 % at most), so that what is rounded on the way is V's product with its scale alone.
+// passes it by more than 2^kLag, so most blocks exchange nothing between lanes.  P enters as two halves, the rounded one and what it left (the matrix cores have the time:
+// +2 % at most): off by 2^-22 of p, or 2^-36 of the row's largest where p is smaller than that allows.  V's product with its scale is one half, 2^-11.
 // Memory-bound: one sequence of 130 000 tokens, 8 KV heads of 128 with 8 query heads each (150 MB): 34 us, 4.4 TB/s; 64 sequences of 0 .. 8192 tokens (306 MB): 70 us,
 // 4.4 TB/s (a large copy moves 4.66).  One sequence of 140 tokens: 7.2 us, latency.
 // The next block's K is fetched into the registers of this one's as soon as its scores are there, its V after the V product: 40 dwords a lane at 128 dims for a
@@ -640,10 +643,10 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
 #pragma unroll
                 for (int e = 1; e < 8; ++e) top = fmaxf(top, s[n][e / 4][e & 3]);
                 top *= sc2[n];
-                if (__ballot(top > mx[n] + 8.0f)) {   // (also the first block: -inf + 8)
+                if (__ballot(top > mx[n] + (kRaise + kLag))) {   // (also the first block: -inf + 15)
                     top = fmaxf(top, lane_xor16(top));
                     top = fmaxf(top, lane_xor32(top));
-                    const float now = fmaxf(mx[n], top);
+                    const float now = fmaxf(mx[n], top - kRaise);
                     const float f = now == -INFINITY ? 1.0f : exp2_fast(mx[n] - now);
                     mx[n] = now;
                     sum[n] *= f;
@@ -833,7 +836,7 @@ template <int NR, bool LINE, int W> __global__ void __launch_bounds__(64 * W) kv
 // V as 16-byte chunks [4 eights of tokens][dim]: both are read and written without bank conflicts.  Two buffers: while one pair of blocks is computed the next is
 // fetched into registers, unpacked and written into the other, one barrier a pair.
 // The row tiles of one (sequence, KV head) go to one XCD, whose L2 then holds that head's codes for all of them; tiles that see most come first.
-// Rounded on the way: K's and V's values and p to halves (2^-11 each at most; the 32 x 32 products want halves).  A float16 result is off by 3.8e-4 of its norm, its own
+// Rounded on the way: K's and V's values and p to halves (2^-11 each at most, p below 2^-25 of the row's largest by up to 2^-36 of that; the 32 x 32 products want halves).  A float16 result is off by 3.8e-4 of its norm, its own
 // rounding alone by 2.1e-4; K exact, as in the kernel above, would take 128 more fused multiply-adds and 32 more LDS reads a step.
 // 2048 tokens, 32 heads of 128 (34 GFLOP): 79 us, 437 TFLOP/s; 4 chunks of up to 512 behind up to 8000 tokens, 64 / 8 heads (234 GFLOP): 372 us, 630 TFLOP/s (a large
 // f16 product: 1142).  Bound by the vector units: 270 instructions a step and wave (exp2 a quarter of their time) take 1300 cycles beside 1024 of matrix products, two
@@ -959,9 +962,9 @@ template <int G> __global__ void __launch_bounds__(256, G <= 4 ? 2 : 1) kv4_prom
 #pragma unroll
         for (int e = 1; e < 32; ++e) top = fmaxf(top, S[e / 16][e & 15]);
         top *= sc2;
-        if (__ballot(top > mx + 8.0f)) {
+        if (__ballot(top > mx + (kRaise + kLag))) {
             top = fmaxf(top, lane_xor32(top));
-            const float now = fmaxf(mx, top);
+            const float now = fmaxf(mx, top - kRaise);
             const float f = now == -INFINITY ? 1.0f : exp2_fast(mx - now);
             mx = now;
             sum *= f;

@@ -1,4 +1,6 @@
 """The 4-bit paged KV cache (ctransformers_amd/ops.py, csrc/engine_kv4.h) at the edges of what its calls accept."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -139,6 +141,38 @@ def test_scores_of_any_size(dev, big, news, scale):
         top = score[:see] == score[:see].max()
         want, mag = vr[:see][top].mean(0), np.abs(vr[:see][top]).mean(0)
         assert (np.abs(got[i] - want) <= mag * 2.0**-10 * 1.01 + np.abs(want) * 2.0**-22).all(), i
+
+
+@pytest.mark.parametrize("news", [1, 20, 200])
+@pytest.mark.parametrize("tail", [24.4, 25.2, 29.0, 35.5])
+@pytest.mark.parametrize("total,parts", [(1024, 0), (1024, 1), pytest.param(60000, 0, marks=pytest.mark.gpu), pytest.param(60000, 1, marks=pytest.mark.gpu)])
+def test_a_peak_and_a_long_flat_tail(dev, total, parts, tail, news):
+    """One token takes all but 2^-tail a token of the weight, and its value is 0: the result is the tail.  Weights are halves, 2^11 times as large as beside a
+    maximum of 1, so the smallest are rounded by 2^-25 2^-11 of the largest at most: sum |v| 2^-36 in the result, beside test_kv4.py's relative roundings (p and v as halves) and its
+    error of a score.  parts: whether the table is wide enough for keys to be divided."""
+    if total > 1024 and dev.type == "cpu":
+        pytest.skip("GPU only (60 000 tokens)")
+    x = torch.tensor(-tail * math.log(2)).half().float()             # (a row with one value has it exactly)
+    for peak in (0, total // 2 + 5, total - news):                   # (every row sees it)
+        pages = torch.zeros((-(-total // 64), ops.kv4_page_bytes(1, 32, 64)), dtype=torch.uint8, device=dev)
+        table = torch.full((1, pages.shape[0] if parts or total > 1024 else 16), -1, dtype=torch.int32, device=dev)
+        table[0, :pages.shape[0]] = torch.arange(pages.shape[0])
+        if parts:
+            table = torch.cat([table, torch.full((1, 200), -1, dtype=torch.int32, device=dev)], 1)
+        k, v = torch.zeros((total, 1, 32)), torch.ones((total, 1, 32))
+        k[:, 0, 0] = x
+        k[peak, 0, 0] = v[peak] = 0
+        n = ints(dev, total)
+        ops.kv4_append(k.to(dev), v.to(dev), pages, table, n, None, total, page_tokens=64)
+        q = torch.zeros((news, 1, 32), dtype=torch.float16)
+        q[..., 0] = 1
+        got = ops.kv4_attention(q.to(dev), pages, table, n, None, news, n_head_kv=1, page_tokens=64, scale=1.0, out=torch.empty(q.shape, dtype=torch.float32, device=dev)).double().cpu()
+        see = torch.arange(total - news + 1, total + 1).double()[:, None, None]
+        w = (see - 1) * math.exp(float(x))
+        want = w / (1 + w)
+        err = (32 + 8) * 2.0**-24 * abs(float(x)) + (4 * abs(float(x)) + 8) * 2.0**-23
+        tol = want * (2 * 2.0**-11 + 2 * math.expm1(err)) * 1.01 + see * 2.0**-36 + want * 2.0**-24 * 1.01
+        assert ((got - want).abs() <= tol).all(), (peak, float(((got - want).abs() / tol).max()))
 
 
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
