@@ -161,9 +161,9 @@ template <int N, class Across> DEV float kv4_query(u32x4 (&q)[N], const Kv4Rows&
                         kv4_cvt2(x[k][6] * up, x[k][7] * up) ^ flip);
     return down;
 }
-// The factor of a score in front of exp2: positive, also for a scale of 0 (whose scores are then as good as equal), so that -inf stays what it is; and at most 2^100,
-// where unequal scores (2^-72 apart at least) have become as far apart as exp2 can tell, and none overflows (below 2^26).
-DEV float kv4_factor(float scale, float down, float unit) { return fminf(fmaxf((fabsf(scale) * down) * (1.44269504088896f * unit), 1e-30f), 0x1p100f); }
+// The factor of a score in front of exp2: positive, also for a scale of 0 (whose scores are then as good as equal), so that -inf stays what it is; and at most 2^86,
+// where unequal scores (2^-72 apart at least) have become further apart than exp2 can tell, and none overflows (float16 queries of 65504 with such keys: 2^40).
+DEV float kv4_factor(float scale, float down, float unit) { return fminf(fmaxf((fabsf(scale) * down) * (1.44269504088896f * unit), 1e-30f), 0x1p86f); }
 // exp2's arguments are fma(score, factor, -maximum): one shift by the rounded maximum for all of a row's weights, which their quotients do not see.  From here on that
 // rounding could carry the largest weight out of the halves' range (and out of exp2's, further up): such rows round the products first, so that the maximum is one of them.
 constexpr float kFar = 0x1p22f;

@@ -117,30 +117,37 @@ def test_queries_at_the_ends_of_their_type(dev, dtype, news):
 @pytest.mark.parametrize("scale", [1.0, -1.0, 3e38])
 @pytest.mark.parametrize("news", [1, 20, 200])
 @pytest.mark.parametrize("big", [2.0**12, 2.0**60, 2.0**126])
-def test_scores_of_any_size(dev, big, news, scale):
+def test_scores_of_any_size(dev, big, news, scale, dtype=torch.float32, key=4096.0):
     """scores beyond 2^30, where a float's steps are larger than the range that exp2 has: the largest takes all, several that are equal share it"""
     width = 10                                       # (in parts too)
     c = Cache(1, [330 + news], 1, 32, 32, extra_width=width)
     pages, table, n = c.on(dev)
     total = 330 + news
     k = torch.zeros((total, 1, 32))
-    k[:, 0, 0] = 4096.0
-    k[:, 0, 1] = 4096.0 * torch.randint(-7, 5, (total,), generator=torch.Generator().manual_seed(5)) / 8   # (exact: a group's largest is 4096, its step 512)
-    k[[3, 77, 300], 0, 1] = -4096.0 if scale < 0 else 4096.0 * 6 / 8
-    k[[3, 77, 300], 0, 0] = -4096.0 if scale < 0 else 4096.0
+    k[:, 0, 0] = key
+    k[:, 0, 1] = key * torch.randint(-7, 5, (total,), generator=torch.Generator().manual_seed(5)) / 8   # (exact: a group's largest is `key`, its step an eighth of it)
+    k[[3, 77, 300], 0, 1] = -key if scale < 0 else key * 6 / 8
+    k[[3, 77, 300], 0, 0] = -key if scale < 0 else key
     v = torch.randn((total, 1, 32), generator=torch.Generator().manual_seed(6))
     ops.kv4_append(k.to(dev), v.to(dev), pages, table, n, None, total, page_tokens=32)
     kr, vr = (x.double().cpu().numpy()[:, 0] for x in ops.kv4_read(pages, table, n, None, total, total, n_head_kv=1, head_dim=32, page_tokens=32, dtype=torch.float32))
-    q = torch.zeros((news, 2, 32), dtype=torch.float32)
+    q = torch.zeros((news, 2, 32), dtype=dtype)
     q[..., 1] = big
     q[..., 0] = big / 4
-    got = ops.kv4_attention(q.to(dev), pages, table, n, None, news, n_head_kv=1, page_tokens=32, scale=scale).double().cpu().numpy()
+    got = ops.kv4_attention(q.to(dev), pages, table, n, None, news, n_head_kv=1, page_tokens=32, scale=scale, out=torch.empty(q.shape, dtype=torch.float32, device=dev)).double().cpu().numpy()
     score = (0.25 * kr[:, 0] + kr[:, 1]) * (1 if scale > 0 else -1)   # times big |scale|: neighbours are 2^20 and more apart
     for i in range(news):
         see = total - news + i + 1
         top = score[:see] == score[:see].max()
         want, mag = vr[:see][top].mean(0), np.abs(vr[:see][top]).mean(0)
         assert (np.abs(got[i] - want) <= mag * 2.0**-10 * 1.01 + np.abs(want) * 2.0**-22).all(), i
+
+
+@pytest.mark.parametrize("scale", [1e37, -3e38])
+@pytest.mark.parametrize("news", [1, 20, 200])
+def test_scores_of_any_size_from_halves(dev, news, scale):
+    """float16 queries go into the products as they are"""
+    test_scores_of_any_size(dev, 2.0**15, news, scale, torch.float16, 32768.0)
 
 
 @pytest.mark.parametrize("news", [1, 20, 200])
