@@ -300,6 +300,19 @@ static bool rows_of(const ctamd_rows* p, Kv4Rows& r, int total, const char*& err
     r.p = p->p; r.row = p->row; r.head = p->head; r.dim = p->dim; r.type = p->type; r.vec = 0;
     return true;
 }
+// Rows that are written: no two elements share memory, shown by each stride reaching past everything that the smaller ones span.
+static bool rows_apart(const Kv4Rows& r, int total, int heads, int dim, const char*& err) {
+    long long size[3] = {total, heads, dim}, step[3] = {r.row < 0 ? -r.row : r.row, r.head < 0 ? -r.head : r.head, r.dim < 0 ? -r.dim : r.dim}, span = 0;
+    for (int i = 0; i < 3; ++i) {
+        int k = -1;
+        for (int j = 0; j < 3; ++j) if (size[j] > 1 && (k < 0 || step[j] < step[k])) k = j;
+        if (k < 0) break;
+        if (step[k] <= span) { err = "two elements of an output share memory"; return false; }
+        span += (size[k] - 1) * step[k];
+        size[k] = 1;
+    }
+    return true;
+}
 static KvPages tables_of(const ctamd_kv_tables* t) {
     KvPages a = KvPages();
     a.table = t->table; a.lens = t->lens; a.refs = t->refs; a.table_o = t->table_out; a.lens_o = t->lens_out; a.refs_o = t->refs_out;
@@ -331,6 +344,7 @@ int ctamd_kv4_read(const ctamd_kv4_cache* cache, const ctamd_rows* k, const ctam
     Kv4Append a = Kv4Append();
     bool ok = cache_of(cache, a.c, err) && rows_of(k, a.k, a.c.total, err) && rows_of(v, a.v, a.c.total, err);
     if (ok && (k->dim != 1 || v->dim != 1)) { err = "the dims of an output row are adjacent"; ok = false; }
+    ok = ok && rows_apart(a.k, a.c.total, a.c.n_head_kv, a.c.head_dim, err) && rows_apart(a.v, a.c.total, a.c.n_head_kv, a.c.head_dim, err);
     ok = ok && ctamd::kv4_read(a, cache->max_rows, (hipStream_t)stream, err);
     return ops_result(ok, "kv4_read", err);
 }
@@ -348,6 +362,7 @@ int ctamd_kv4_attention(const ctamd_kv4_cache* cache, int n_head, const ctamd_ro
     Kv4Rows o = Kv4Rows();
     bool ok = cache_of(cache, a.c, err) && rows_of(q, a.q, a.c.total, err) && rows_of(out, o, a.c.total, err);
     if (ok && o.dim != 1) { err = "the dims of an output row are adjacent"; ok = false; }
+    ok = ok && rows_apart(o, a.c.total, n_head, a.c.head_dim, err);
     a.out = (void*)o.p; a.o_row = o.row; a.o_head = o.head; a.out_type = o.type; a.n_head = n_head; a.scale = scale; a.ws = ws;
     ok = ok && ctamd::kv4_attention(a, cache->max_rows, ws_floats, (hipStream_t)stream, err);
     return ops_result(ok, "kv4_attention", err);

@@ -190,7 +190,7 @@ def kv4_attention(q, pages, table, lens, cu, max_rows, *, n_head_kv, page_tokens
     """Causal attention of the rows q [total, n_head, head_dim] over the cache: row i of a sequence with n rows sees the positions 0 .. lens - n + i, query head h
     reads KV head h // (n_head / n_head_kv), scores are q.k * scale (finite; default 1 / sqrt(head_dim)).  A row that sees nothing becomes 0.  q is float16, bfloat16 or
     float32; the result has q's type, or is written into `out` [total, n_head, head_dim] of any of the three, where rows that belong to no sequence are left as they
-    are.  Products are taken in float16 (K's codes and V's values; q scaled by a power of two per row, and p), everything else in float32."""
+    are; `out` may be q itself, but shares no memory with any other tensor of the call, nor any two of its own elements.  Products are taken in float16 (K's codes and V's values; q scaled by a power of two per row, and p), everything else in float32."""
     device = _device_of("pages", pages)
     qr = _rows(device, "q", q)
     total, n_head, head_dim = q.shape

@@ -39,10 +39,11 @@ typedef struct {
 } ctamd_rows;
 /* Quantizes K and V rows [total][n_head_kv][head_dim] into the pages.  A token whose K or V of a head holds a NaN makes every row that sees it NaN. */
 int ctamd_kv4_append(const ctamd_kv4_cache* cache, const ctamd_rows* k, const ctamd_rows* v, void* stream);
-/* The last rows of every sequence as numbers (0 where there is no page or no position). */
+/* The last rows of every sequence as numbers (0 where there is no page or no position).  No two elements of k and v are the same memory. */
 int ctamd_kv4_read(const ctamd_kv4_cache* cache, const ctamd_rows* k, const ctamd_rows* v, void* stream);
 /* Causal attention of rows [total][n_head][head_dim] over the cache: row i of a sequence with n rows sees positions 0 .. lens - n + i; a row that sees nothing
- * becomes 0.  n_head is a multiple of n_head_kv, dims of q are adjacent (q.dim == out.dim == 1), scale is finite.  Rows that belong to no sequence are left as they are.
+ * becomes 0.  n_head is a multiple of n_head_kv, dims of q are adjacent (q.dim == out.dim == 1), scale is finite; out may be q itself, but shares no
+ * memory with anything else, and no two of its elements are the same memory.  Rows that belong to no sequence are left as they are.
  * ws: ctamd_kv4_attention_ws() floats (a function of the sizes alone, 0 if none are wanted), 16-byte aligned. */
 long long ctamd_kv4_attention_ws(const ctamd_kv4_cache* cache, int n_head);
 int ctamd_kv4_attention(const ctamd_kv4_cache* cache, int n_head, const ctamd_rows* q, const ctamd_rows* out, float scale, float* ws, long long ws_floats,

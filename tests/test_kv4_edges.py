@@ -182,6 +182,40 @@ def test_a_peak_and_a_long_flat_tail(dev, total, parts, tail, news):
         assert ((got - want).abs() <= tol).all(), (peak, float(((got - want).abs() / tol).max()))
 
 
+@pytest.mark.parametrize("news", [1, 20, 200])
+def test_results_in_the_queries_place(dev, news):
+    c = Cache(1, [300 + news, 20], 2, 32, 32, extra_width=12)
+    c.fill(2)
+    pages, table, lens = c.on(dev)
+    q = torch.randn((news + 3, 10, 32), generator=torch.Generator().manual_seed(1)).half().to(dev)
+    att = lambda out: ops.kv4_attention(q, pages, table, lens, ints(dev, 0, news, news + 3), news, n_head_kv=2, page_tokens=32, out=out)  # noqa: E731
+    want = att(None)
+    assert torch.equal(att(q), want)
+
+
+def test_results_whose_rows_share_memory(dev):
+    """refused, rows that lie between others are not"""
+    c = Cache(1, [40], 1, 32, 32)
+    c.fill(2)
+    pages, table, lens = c.on(dev)
+    q = torch.randn((5, 4, 32), generator=torch.Generator().manual_seed(1)).half().to(dev)
+    att = lambda out: ops.kv4_attention(q, pages, table, lens, None, 5, n_head_kv=1, page_tokens=32, out=out)  # noqa: E731
+    want = att(None)
+    flat = torch.full((4000,), 7.0, dtype=torch.float16, device=dev)
+    for size, stride in (((5, 4, 32), (0, 32, 1)), ((5, 4, 32), (128, 0, 1)), ((5, 4, 32), (64, 32, 1)), ((5, 4, 32), (128, 24, 1)), ((5, 4, 32), (16, 160, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            att(flat.as_strided(size, stride))
+    assert (flat == 7).all()
+    for stride in ((128, 32, 1), (40, 208, 1), (160, 40, 1), (700, 33, 1)):
+        flat.fill_(7)
+        assert torch.equal(att(flat.as_strided((5, 4, 32), stride)), want)
+        assert int((flat != 7).sum()) <= 640
+    row = lambda *s: ops.ROWS.pack(flat.data_ptr(), *s, 0)  # noqa: E731
+    cache = ops.CACHE.pack(pages.data_ptr(), table.data_ptr(), lens.data_ptr(), 0, pages.stride(0), pages.shape[0], table.shape[1], table.shape[1], 1, 5, 1, 32, 32, 5)
+    for k, v in ((row(0, 32, 1), row(32, 32, 1)), (row(32, 32, 1), row(16, 32, 1))):
+        assert ops._lib.ctamd_kv4_read(cache, k, v, None) == -1 and b"share memory" in ops._lib.ctamd_ops_error()
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("length,add", [(2**31 - 1, 2**31 - 1), (1, 2**31 - 1), (2**31 - 1, 1), (2**30, 2**30)])
 def test_room_behind_lengths_near_2_31(dev, length, add):
