@@ -23,12 +23,22 @@ long long kv4_page_bytes(int n_head_kv, int head_dim, int page_tokens) {
     return (long long)n_head_kv * (page_tokens / 32) * g * kKv4Block;
 }
 
-static bool launched(const char*& err) {
-    const hipError_t e = hipGetLastError();
-    if (e == hipSuccess) return true;
-    err = hipGetErrorString(e);
-    return false;
+// Queues a kernel; false if THIS launch failed.  (What hipGetLastError says may be left from another call of the thread, and stays there for its owner.)
+template <class T> struct Plain { typedef T type; };
+#ifdef CT_EMU
+template <class... P> static bool queue(const char*&, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, hipStream_t stream, typename Plain<P>::type... p) {
+    (void)stream;
+    CT_LAUNCH_DYN(kernel, grid, block, smem, stream, p...);
+    return true;
 }
+#else
+template <class... P> static bool queue(const char*& err, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, hipStream_t stream, typename Plain<P>::type... p) {
+    void* args[] = {&p...};
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, args, smem, stream);
+    if (e != hipSuccess) err = hipGetErrorString(e);
+    return e == hipSuccess;
+}
+#endif
 // the dynamic LDS of a kernel beyond 64 KB has to be allowed, once per device
 #define KV4_OPTIN(fn, bytes) \
     do { if ((bytes) > 64 * 1024) (void)CT_SMEM_OPTIN(fn, bytes); } while (0)
@@ -87,16 +97,16 @@ bool kv4_append(Kv4Append& a, int max_rows, hipStream_t stream, const char*& err
     dim3 grid;
     if (a.c.total == 0 || a.c.n_seq == 0 || a.c.n_pages == 0 || max_rows <= 0) return true;
     if (!append_grid(a, max_rows, grid, err)) return false;
-    KV4_BY_GROUPS(a.c.groups, CT_LAUNCH(kv4_append_kernel<G>, grid, dim3(256), stream, a);)
-    return launched(err);
+    KV4_BY_GROUPS(a.c.groups, return queue(err, kv4_append_kernel<G>, grid, dim3(256), 0, stream, a);)
+    return true;
 }
 
 bool kv4_read(Kv4Append& a, int max_rows, hipStream_t stream, const char*& err) {
     dim3 grid;
     if (a.c.total == 0 || a.c.n_seq == 0 || max_rows <= 0) return true;
     if (!tables_there(a.c, err) || !append_grid(a, max_rows, grid, err)) return false;
-    KV4_BY_GROUPS(a.c.groups, CT_LAUNCH(kv4_read_kernel<G>, grid, dim3(256), stream, a);)
-    return launched(err);
+    KV4_BY_GROUPS(a.c.groups, return queue(err, kv4_read_kernel<G>, grid, dim3(256), 0, stream, a);)
+    return true;
 }
 
 // Rows of a tile: kv4_decode_kernel takes 16, or 32 where two tiles of a head fit the registers (128 dims), kv4_prompt_kernel 128.  The first streams the codes at
@@ -152,22 +162,19 @@ long long kv4_attention_plan(Kv4Attn& a, int max_rows) {
     return split > 1 ? units * split * tr * (c.head_dim + 2) : 0;
 }
 
-template <int G, int NT> static void launch_decode(const Kv4Attn& a, hipStream_t stream) {
+template <int G, int NT> static bool launch_decode(const Kv4Attn& a, hipStream_t stream, const char*& err) {
     constexpr size_t smem = (size_t)(4 * 16 * (32 * G + 4) + 4 * 16 * NT * 2) * 4;
     auto kfn = kv4_decode_kernel<G, NT>;
     KV4_OPTIN(kfn, smem);
     const long long units = (long long)a.c.n_seq * a.c.n_head_kv * a.tiles, n = a.nsplit > 1 ? shares(a, units, (long long)a.c.table_width << a.c.bshift) : units;
-    CT_LAUNCH_DYN(kfn, dim3((unsigned)n), dim3(256), smem, stream, a);
+    return queue(err, kfn, dim3((unsigned)n), dim3(256), smem, stream, a);
 }
 
-template <int W> static void launch_join(const Kv4Attn& a, int tr, dim3 grid, hipStream_t stream) {
-    if (tr < 128) {
-        if (a.c.head_dim <= 128) CT_LAUNCH((kv4_join_kernel<1, true, W>), grid, dim3(64 * W), stream, a, tr);
-        else CT_LAUNCH((kv4_join_kernel<2, true, W>), grid, dim3(64 * W), stream, a, tr);
-    } else {
-        if (a.c.head_dim <= 128) CT_LAUNCH((kv4_join_kernel<1, false, W>), grid, dim3(64 * W), stream, a, tr);
-        else CT_LAUNCH((kv4_join_kernel<2, false, W>), grid, dim3(64 * W), stream, a, tr);
-    }
+template <int W> static bool launch_join(const Kv4Attn& a, int tr, dim3 grid, hipStream_t stream, const char*& err) {
+    const dim3 block(64 * W);
+    if (tr < 128)
+        return a.c.head_dim <= 128 ? queue(err, kv4_join_kernel<1, true, W>, grid, block, 0, stream, a, tr) : queue(err, kv4_join_kernel<2, true, W>, grid, block, 0, stream, a, tr);
+    return a.c.head_dim <= 128 ? queue(err, kv4_join_kernel<1, false, W>, grid, block, 0, stream, a, tr) : queue(err, kv4_join_kernel<2, false, W>, grid, block, 0, stream, a, tr);
 }
 
 bool kv4_attention(Kv4Attn& a, int max_rows, long long ws_floats, hipStream_t stream, const char*& err) {
@@ -184,30 +191,28 @@ bool kv4_attention(Kv4Attn& a, int max_rows, long long ws_floats, hipStream_t st
     if (pairs * a.tiles * (((long long)c.table_width << c.bshift) + kUnitCost) > 0x7FFFFFFF) { err = "a table with room for 2^31 blocks or more over all heads"; return false; }
     if (grid > 0x7FFFFFFF || (long long)c.total * a.n_head > 0x7FFFFFFF) { err = "too many rows times sequences for one call"; return false; }
     const int tr = tile_rows(a, (long long)(max_rows > c.total ? c.total : max_rows) * a.rep);
+    bool ok = false;
     if (tr == 16) {
-        KV4_BY_GROUPS(c.groups, (launch_decode<G, 1>(a, stream));)
+        KV4_BY_GROUPS(c.groups, (ok = launch_decode<G, 1>(a, stream, err));)
     } else if (tr == 32) {
         switch (c.groups) {
-            case 1: launch_decode<1, 2>(a, stream); break;
-            case 2: launch_decode<2, 2>(a, stream); break;
-            case 3: launch_decode<3, 2>(a, stream); break;
-            default: launch_decode<4, 2>(a, stream); break;
+            case 1: ok = launch_decode<1, 2>(a, stream, err); break;
+            case 2: ok = launch_decode<2, 2>(a, stream, err); break;
+            case 3: ok = launch_decode<3, 2>(a, stream, err); break;
+            default: ok = launch_decode<4, 2>(a, stream, err); break;
         }
     } else {
         KV4_BY_GROUPS(c.groups, {
             auto kfn = kv4_prompt_kernel<G>;
             constexpr size_t smem = Kv4Lds<G>::BYTES;
             KV4_OPTIN(kfn, smem);
-            CT_LAUNCH_DYN(kfn, dim3((unsigned)grid), dim3(256), smem, stream, a);
+            ok = queue(err, kfn, dim3((unsigned)grid), dim3(256), smem, stream, a);
         })
     }
-    if (a.nsplit > 1) {
-        const dim3 jg((unsigned)((long long)c.total * a.n_head));
-        // few rows: eight waves for each, their parts are many; many rows: a wave each, all of them resident at once
-        if ((long long)c.total * a.n_head <= 2048) launch_join<8>(a, tr, jg, stream);
-        else launch_join<1>(a, tr, jg, stream);
-    }
-    return launched(err);
+    if (!ok || a.nsplit <= 1) return ok;
+    const dim3 jg((unsigned)((long long)c.total * a.n_head));
+    // few rows: eight waves for each, their parts are many; many rows: a wave each, all of them resident at once
+    return (long long)c.total * a.n_head <= 2048 ? launch_join<8>(a, tr, jg, stream, err) : launch_join<1>(a, tr, jg, stream, err);
 }
 
 // ---- pages ------------------------------------------------------------------------------------------------------------------------------------------
@@ -254,27 +259,24 @@ bool kv_fork(const KvPages& a, hipStream_t stream, const char*& err) {
     if (!pages_check(a, true, err)) return false;
     if (a.n_new && !a.parents) { err = "null parents"; return false; }
     const long long cells = (long long)a.n_new * a.width;
-    CT_LAUNCH(kv_fork_rows_kernel, dim3(groups_for(cells > a.n_pages ? cells : a.n_pages, 256, 2048)), dim3(256), stream, a);
+    if (!queue(err, kv_fork_rows_kernel, dim3(groups_for(cells > a.n_pages ? cells : a.n_pages, 256, 2048)), dim3(256), 0, stream, a)) return false;
     const int rows = a.n_seq + (a.keep ? a.n_new : 0);
-    if (rows) CT_LAUNCH(kv_fork_counts_kernel, dim3((unsigned)rows), dim3(256), stream, a);
-    return launched(err);
+    return !rows || queue(err, kv_fork_counts_kernel, dim3((unsigned)rows), dim3(256), 0, stream, a);
 }
 bool kv_reserve(const KvPages& a, hipStream_t stream, const char*& err) {
     if (!pages_check(a, true, err) || !move_check(a, err)) return false;
     if (a.n_seq && !a.add) { err = "null add"; return false; }
     const long long cells = (long long)a.n_seq * a.width;
-    CT_LAUNCH(kv_reserve_plan_kernel, dim3(1 + groups_for(cells > a.n_pages ? cells : a.n_pages, kPlanThreads, 256)), dim3(kPlanThreads), stream, a);
+    if (!queue(err, kv_reserve_plan_kernel, dim3(1 + groups_for(cells > a.n_pages ? cells : a.n_pages, kPlanThreads, 256)), dim3(kPlanThreads), 0, stream, a)) return false;
     const unsigned apply = groups_for(a.n_seq, 4, 256);
-    CT_LAUNCH(kv_reserve_apply_kernel, dim3(apply + movers(a, a.n_seq)), dim3(256), stream, a, (int)apply);
-    return launched(err);
+    return queue(err, kv_reserve_apply_kernel, dim3(apply + movers(a, a.n_seq)), dim3(256), 0, stream, a, (int)apply);
 }
 bool kv_compact(const KvPages& a, hipStream_t stream, const char*& err) {
     if (!pages_check(a, false, err) || !move_check(a, err)) return false;
     const long long cells = (long long)a.n_seq * a.width;
-    CT_LAUNCH(kv_compact_plan_kernel, dim3(1), dim3(kPlanThreads), stream, a);
+    if (!queue(err, kv_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a)) return false;
     const unsigned apply = groups_for(cells > a.n_pages ? cells : a.n_pages, 256, 256);
-    CT_LAUNCH(kv_compact_apply_kernel, dim3(apply + movers(a, a.n_pages / 2)), dim3(256), stream, a, (int)apply);
-    return launched(err);
+    return queue(err, kv_compact_apply_kernel, dim3(apply + movers(a, a.n_pages / 2)), dim3(256), 0, stream, a, (int)apply);
 }
 
 }  // namespace ctamd

@@ -2,7 +2,7 @@
  * ctransformers_amd/ops.py calls these with torch tensors; a handle created with CT_AMD_KV=q4 runs its own attention on the same kernels.
  *
  * Conventions.  Every pointer but `stream` (a hipStream_t, NULL: the default stream) names memory of the CURRENT device.  A call only queues work on `stream`
- * and returns 0, or -1 (nothing queued; ctamd_ops_error() says why, per thread).  Nothing is kept between calls and no call allocates, copies to the host or waits,
+ * and returns 0, or -1; ctamd_ops_error() says why, per thread: arguments are refused before anything is queued, a launch that the runtime refuses ends the call there.  Nothing is kept between calls and no call allocates, copies to the host or waits,
  * so all of them can be captured into a graph; two calls at once need two workspaces.
  *
  * Row types: 0 fp16, 1 bf16, 2 fp32.  Strides count elements.  A cache is

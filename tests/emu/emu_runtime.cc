@@ -4,6 +4,8 @@
 #include <vector>
 
 dim3 threadIdx, blockIdx, blockDim, gridDim;
+int emu_last_error = 0;
+extern "C" int emu_get_last_error() { const int e = emu_last_error; emu_last_error = 0; return e; }
 
 namespace emu {
 namespace {

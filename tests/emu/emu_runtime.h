@@ -95,7 +95,9 @@ static inline hipError_t hipMemcpyPeerAsync(void* d, int, const void* s, int, si
 static inline hipError_t hipDeviceCanAccessPeer(int* can, int, int) { *can = 1; return hipSuccess; }
 static inline hipError_t hipDeviceEnablePeerAccess(int, unsigned) { return hipSuccess; }
 static inline hipError_t hipDeviceSynchronize() { return hipSuccess; }
-static inline hipError_t hipGetLastError() { return hipSuccess; }
+extern "C" int emu_last_error;          // 0, or the error that a call of the thread left (tests set it)
+extern "C" int emu_get_last_error();    // that, and 0 from then on
+static inline hipError_t hipGetLastError() { return emu_get_last_error(); }
 template <class P> static inline hipError_t hipMalloc(P** p, size_t n) { return hipMalloc((void**)p, n); }
 template <class P> static inline hipError_t hipHostMalloc(P** p, size_t n, unsigned f = 0) { return hipHostMalloc((void**)p, n, f); }
 

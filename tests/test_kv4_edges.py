@@ -1,4 +1,5 @@
 """The 4-bit paged KV cache (ctransformers_amd/ops.py, csrc/engine_kv4.h) at the edges of what its calls accept."""
+import ctypes
 import math
 
 import numpy as np
@@ -214,6 +215,34 @@ def test_results_whose_rows_share_memory(dev):
     cache = ops.CACHE.pack(pages.data_ptr(), table.data_ptr(), lens.data_ptr(), 0, pages.stride(0), pages.shape[0], table.shape[1], table.shape[1], 1, 5, 1, 32, 32, 5)
     for k, v in ((row(0, 32, 1), row(32, 32, 1)), (row(32, 32, 1), row(16, 32, 1))):
         assert ops._lib.ctamd_kv4_read(cache, k, v, None) == -1 and b"share memory" in ops._lib.ctamd_ops_error()
+
+
+def test_an_error_that_another_call_left(dev):
+    """it is not this call's, and stays there for its owner"""
+    pages, table, lens, refs = torch.zeros((2, ops.kv4_page_bytes(1, 32, 32)), dtype=torch.uint8, device=dev), ints(dev, [0, -1]), ints(dev, 1), ints(dev, 1, 0)
+    x = torch.ones((1, 1, 32), device=dev)
+    if dev.type == "cpu":
+        word = ctypes.c_int.in_dll(ops._lib, "emu_last_error")
+        leave, take = lambda: setattr(word, "value", 101), ops._lib.emu_get_last_error
+    else:
+        hip = ctypes.CDLL(next(line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line))
+        leave, take = lambda: hip.hipSetDevice(10**6), hip.hipGetLastError
+    parents = ints(dev, 0)
+    for _ in range(2):   # (kernels are loaded, memory has been taken)
+        ops.kv4_append(x, x, pages, table, lens, None, 1, page_tokens=32)
+        out = ops.kv4_attention(x, pages, table, lens, None, 1, n_head_kv=1, page_tokens=32)
+        ops.kv_fork(table, lens, refs, parents, page_tokens=32)
+    take()
+    leave()
+    try:
+        ops.kv4_append(x, x, pages, table, lens, None, 1, page_tokens=32)
+        assert take() == 101
+        leave()
+        out = ops.kv4_attention(x, pages, table, lens, None, 1, n_head_kv=1, page_tokens=32)
+        ops.kv_fork(table, lens, refs, parents, page_tokens=32)
+    finally:
+        take()
+    assert (out == 1).all()
 
 
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
