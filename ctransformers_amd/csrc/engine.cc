@@ -560,8 +560,13 @@ void Engine::fill_attn_args(AttnArgsX& ax, uint16_t* kc, uint16_t* vc, int nt) {
 
 #include "engine_kv4.h"
 
+bool Engine::attend(uint16_t* kc, uint16_t* vc, int nt, std::string& err) {
+    if (kv4_) return kv4_attend(kc, vc, nt, err);
+    launch_attention(kc, vc, nt);
+    return true;
+}
+
 void Engine::launch_attention(uint16_t* kc, uint16_t* vc, int nt) {
-    if (kv4_) { kv4_attend(kc, vc, nt); return; }
     const int hd = hp_.head_dim();
     AttnArgsX ax = AttnArgsX();
     fill_attn_args(ax, kc, vc, nt);
@@ -1067,6 +1072,7 @@ bool Engine::run_chunk(int c0, int nt, bool want_logits, std::string& err) {
 bool Engine::ensure_graphs(std::string& err) {
 #ifndef CT_EMU
     if (graph_step_) return true;
+    hipGraphExec_t step[2] = {nullptr, nullptr};   // (both or neither: a capture that fails leaves the handle without graphs)
     for (int head = 0; head < 2; ++head) {
         hipGraph_t g = nullptr;
         std::unique_lock<std::recursive_mutex> cap(capture_mutex());
@@ -1074,13 +1080,13 @@ bool Engine::ensure_graphs(std::string& err) {
         const bool ok = token_step(head == 1, err);
         hipError_t e = hipStreamEndCapture(stream_, &g);
         cap.unlock();
-        if (!ok) { if (g) (void)hipGraphDestroy(g); return false; }
-        if (e != hipSuccess) { err = std::string("hipStreamEndCapture failed: ") + hipGetErrorString(e); return false; }
-        hipGraphExec_t ex = nullptr;
-        HIP_OK(hipGraphInstantiate(&ex, g, nullptr, nullptr, 0));
-        HIP_OK(hipGraphDestroy(g));
-        (head ? graph_step_head_ : graph_step_) = ex;
+        if (ok && e != hipSuccess) err = std::string("hipStreamEndCapture failed: ") + hipGetErrorString(e);
+        else if (ok && (e = hipGraphInstantiate(&step[head], g, nullptr, nullptr, 0)) != hipSuccess) err = std::string("hipGraphInstantiate failed: ") + hipGetErrorString(e);
+        if (g) (void)hipGraphDestroy(g);
+        if (!ok || e != hipSuccess) { if (head && step[0]) (void)hipGraphExecDestroy(step[0]); return false; }
     }
+    graph_step_ = step[0];
+    graph_step_head_ = step[1];
     // continuation steps of a greedy chain: no embedding launch (the previous head launch left the row, the token id and the cursor),
     // outputs into pair member b
     if (spec_possible()) {
@@ -1320,7 +1326,6 @@ bool Engine::req_wait(int n, int n_past, std::string& err) {
               "its own grid (is the device shared?): the request is evaluated again with the forms that need no residency";
         return false;
     }
-    if (!kv4_err_.empty()) { err = kv4_err_; kv4_err_.clear(); return false; }
     have_logits_ = l1_ == hp_.n_layer;
     last_token_ = h_scalars_[4 + n - 1];
     last_pos_ = n_past + n - 1;

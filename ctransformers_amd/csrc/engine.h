@@ -193,9 +193,10 @@ class Engine {
     bool mm8_can(const ::MatvecArgs& m) const;   // every job of the site has a LAYOUT_M8 arena the order-free kernels take (kernels_mm8.h)
     bool mm8_matvec(::MatvecArgs& m, const float* x, int ldx, int nt, int ld_out, int ld_res, std::string& err);
     void launch_attention(uint16_t* kc, uint16_t* vc, int nt = 0);
+    bool attend(uint16_t* kc, uint16_t* vc, int nt, std::string& err);   // the fp16 cache or the 4-bit one
     bool kv4_setup(std::string& err);
     bool kv4_cache(::Kv4Cache& c, int layer, int rows, const char*& why);
-    void kv4_attend(const uint16_t* kc, const uint16_t* vc, int nt);
+    bool kv4_attend(const uint16_t* kc, const uint16_t* vc, int nt, std::string& err);
     bool kv4_tables(bool reserve, std::string& err);
     bool kv4_row(std::string& err);
     bool kv4_room(int n_past, int n, std::string& err);
@@ -246,7 +247,6 @@ class Engine {
     int *kv_table_[2] = {nullptr, nullptr}, *kv_lens_[2] = {nullptr, nullptr}, *kv_refs_[2] = {nullptr, nullptr};
     int *kv_row_ = nullptr, *kv_args_ = nullptr, *kv_ws_ = nullptr, *h_kv_ = nullptr;
     float* kv_attn_ws_ = nullptr;
-    std::string kv4_err_;
     float *x_ = nullptr, *attn_out_ = nullptr, *h_ = nullptr, *scores_ = nullptr, *d_logits_ = nullptr, *d_emb_ = nullptr;
     float* f16_tmp_ = nullptr;   // models with F16 weight matrices: raw rows of one mat-vec site (kernels_f16.h)
     bool has_raw_ = false;   // some matrix stays in file layout (F16, Q4_1, Q5_0, Q5_1): two-launch sites, token steps only
@@ -320,6 +320,7 @@ class Engine {
     int cur_layer_ = 0;               // layer whose launches are being issued (tags of the in-launch exchanges)
     long long qa_launches_ = 0;
     long long resident_replays_ = 0;   // requests evaluated a second time after a residency give-up
+    int dbg_kv4_fail_ = 0;             // tests (CT_AMD_DBG_KV4_FAIL=N): the N-th attention launch of this handle over the 4-bit cache is refused
     int dbg_qa_timeout_ = 0;           // tests (CT_AMD_DBG_QA_TIMEOUT=N): the N-th wait of this handle behaves as if a sweep had given up
     unsigned* pick_ws_ = nullptr;     // head launch: one 64-bit key per wave, [workgroup][16] (kernels_v9.h:v9_pick_store)
     int cur_buf_ = 0;

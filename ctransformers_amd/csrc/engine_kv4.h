@@ -17,6 +17,7 @@ bool Engine::kv4_setup(std::string& err) {
         return true;
     }
     if (hp_.legacy() || l0_ != 0 || l1_ != hp_.n_layer) { err = "CT_AMD_KV=q4 serves llama and falcon models on one GPU"; return false; }
+    dbg_kv4_fail_ = env_int("CT_AMD_DBG_KV4_FAIL", 0);
     if (n > 256) { err = "CT_AMD_CONTEXTS: at most 256"; return false; }
     ctxs_.assign((size_t)n, Context());
     kv_page_ = env_int("CT_AMD_KV_PAGE", 64);
@@ -62,7 +63,7 @@ bool Engine::kv4_cache(Kv4Cache& c, int layer, int rows, const char*& why) {
 }
 
 // the layer's rows of this step from the fp16 buffers into its pages, then attention over the pages
-void Engine::kv4_attend(const uint16_t* kc, const uint16_t* vc, int nt) {
+bool Engine::kv4_attend(const uint16_t* kc, const uint16_t* vc, int nt, std::string& err) {
     const int rows = std::max(1, nt), hd = hp_.head_dim();
     const char* why = nullptr;
     Kv4Append ap = Kv4Append();
@@ -78,9 +79,11 @@ void Engine::kv4_attend(const uint16_t* kc, const uint16_t* vc, int nt) {
     at.q.p = ax.q_f16; at.q.row = ax.q_stride; at.q.head = hd; at.q.dim = 1; at.q.type = KV4_F16;
     at.out = ax.out; at.o_row = ax.out_stride; at.o_head = hd; at.out_type = KV4_F32;
     at.n_head = hp_.n_head; at.scale = ax.kq_scale; at.ws = kv_attn_ws_;
+    if (dbg_kv4_fail_ > 0 && --dbg_kv4_fail_ == 0) { ok = false; why = "refused on purpose"; }
     ok = ok && kv4_attention(at, rows, kv_attn_ws_n_, stream_, why);
-    if (!ok && kv4_err_.empty()) kv4_err_ = std::string("attention over the 4-bit cache: ") + (why ? why : "launch failed");
+    if (!ok) { err = std::string("attention over the 4-bit cache: ") + (why ? why : "launch failed"); return false; }   // (a step without it is no step: nor is a graph of it)
     ++kv4_launches_;
+    return true;
 }
 
 // One change of the tables: the two (n) vectors in kv_args_ — parents and kept lengths of a fork, or the tokens to make room for — are on their way; the call's

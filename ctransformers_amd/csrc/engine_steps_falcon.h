@@ -39,7 +39,7 @@ bool Engine::chunk_step_falcon(int c0, int nt, bool want_logits, std::string& er
             CT_LAUNCH(falcon_rope_store_kernel, dim3((unsigned)(hp_.n_head + 2 * hp_.n_head_kv), (unsigned)nt), dim3((unsigned)(hd / 2)), stream_,
                       (const float*)qkv_tmp_b_, q_f16_b_, kc, vc, (const float*)rope_cs_, d_pos, hp_.n_head, hp_.n_head_kv, hd, n_ctx_,
                       v_stride_, falcon_fold_ ? 1 : 0);
-        if (site_on("attn_fused")) launch_attention(kc, vc, nt);
+        if (site_on("attn_fused") && !attend(kc, vc, nt, err)) return false;
         {   // Wo, kept apart: the residual is added after the MLP
             MatvecArgs a = base;
             a.K = E; a.pro = PRO_PLAIN; a.out = attn_proj_b_;
@@ -144,7 +144,7 @@ bool Engine::token_step_falcon(bool want_logits, std::string& err) {
         }
         if (!fused_qa && site_on("attn_fused")) {
             prof_begin("attn_fused", "attn_fused_exact_kernel", 0.0);
-            launch_attention(kc, vc);
+            if (!attend(kc, vc, 0, err)) return false;
             prof_end();
         }
         {   // Q8_K(attn) -> Wo  (kept apart: the residual is added after the MLP)

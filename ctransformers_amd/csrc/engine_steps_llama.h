@@ -38,7 +38,7 @@ bool Engine::chunk_step(int c0, int nt, bool want_logits, std::string& err) {
         }
         if (site_on("attn_fused")) {
             prof_begin("attn_fused", "attn_fused_exact_kernel", 0.0);
-            launch_attention(kc, vc, nt);
+            if (!attend(kc, vc, nt, err)) return false;
             prof_end();
         }
         {
@@ -140,7 +140,7 @@ bool Engine::token_step(bool want_logits, std::string& err) {
                 if (stamps_ && stamps_level_ > 1) CT_LAUNCH(stamp_kernel, dim3(1), dim3(1), stream_, stamps_, 3ull);
                 if (site_on("attn_fused")) {
                     prof_begin("attn_fused", "attn_fused_exact_kernel", 0.0);
-                    launch_attention(kc, vc);
+                    if (!attend(kc, vc, 0, err)) return false;
                     prof_end();
                 }
                 debug_dump("2attn", il);

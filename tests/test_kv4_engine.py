@@ -207,3 +207,31 @@ def test_refusals(lib, monkeypatch, capfd):
         plain.use_context(0)
     with pytest.raises(RuntimeError):
         plain.compact_contexts()
+
+
+@pytest.mark.parametrize("nth", [1, 3, 5, 7, 9, 12])
+def test_a_refused_attention_launch_fails_every_eval_that_would_lack_it(lib, nth, monkeypatch):
+    """The nth attention launch of the handle is refused (two layers; on the GPU: the load's warm-up, the captures of the token steps, an eager chunk, a chunk's capture, ..).
+    The load or the eval that issues it fails; whatever succeeds afterwards has all its launches: no graph without the launch stays behind."""
+    path = os.path.join(GOLDEN, "tiny-q4km.gguf")
+    toks = [int(t) for t in np.random.default_rng(3).integers(3, 200, 12)]
+    plain = open_model(path, lib, monkeypatch, ctx=64)
+    failed = 0
+    try:
+        m = open_model(path, lib, monkeypatch, ctx=64, CT_AMD_DBG_KV4_FAIL=nth)
+    except RuntimeError:
+        assert lib == HIP_LIB
+        return
+    steps = [toks[:3], toks[3:6], toks[6:9], toks[9:10], toks[10:11]] if lib == HIP_LIB else [toks[:2], toks[2:3]]
+    for step in steps:
+        for _ in range(2):
+            plain._context[:] = m._context
+            try:
+                m.eval(step)
+            except RuntimeError:
+                failed += 1
+                continue
+            plain.eval(step)
+            assert np.array_equal(m.logits.to_numpy(), plain.logits.to_numpy())
+            break
+    assert failed == (nth <= (10 if lib == HIP_LIB else 4))
