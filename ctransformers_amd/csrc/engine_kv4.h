@@ -156,6 +156,7 @@ bool Engine::context_fork(int src, int dst, std::string& err) {
     HIP_OK(hipSetDevice(device_));
     for (int i = 0; i < m; ++i) { h_kv_[i] = i == dst ? src : i; h_kv_[m + i] = i == dst ? ctxs_[src].len : 0x7FFFFFFF; }
     if (!kv4_tables(false, err)) return false;
+    if (src == active_ || dst == active_) last_pos_ = -1;   // (its page is shared now, or what it was the last token of is gone: not to be written again by a measurement)
     const int len = ctxs_[src].len, shared = (len + kv_page_ - 1) / kv_page_ * kv_page_;
     ctxs_[src].own_from = std::max(ctxs_[src].own_from, shared);
     ctxs_[dst] = Context{len, len, shared};
@@ -168,6 +169,7 @@ bool Engine::context_free(int i, std::string& err) {
     for (int k = 0; k < m; ++k) { h_kv_[k] = k == i ? -1 : k; h_kv_[m + k] = 0x7FFFFFFF; }
     if (!kv4_tables(false, err)) return false;
     ctxs_[i] = Context();
+    if (i == active_) last_pos_ = -1;
     return kv4_row(err);
 }
 int Engine::context_compact(std::string& err) {   // pages in use, -1: failed

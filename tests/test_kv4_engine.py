@@ -11,6 +11,7 @@ import pytest
 
 from conftest import HIP_LIB, ROOT, has_gpu
 from ctransformers_amd.llm import LLM, Config
+from ctransformers_amd.measure import LaunchStat
 from test_kv4 import attention64, quantize
 from tools import synth
 
@@ -235,3 +236,30 @@ def test_a_refused_attention_launch_fails_every_eval_that_would_lack_it(lib, nth
             assert np.array_equal(m.logits.to_numpy(), plain.logits.to_numpy())
             break
     assert failed == (nth <= (10 if lib == HIP_LIB else 4))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("active", [0, 1])
+def test_measurements_do_not_write_into_pages_that_a_fork_shares(hip_lib, active, monkeypatch):
+    """a measurement replays the last token of the active context; after a fork that position lies in the other context's pages too (or was dropped): there is nothing to replay"""
+    path = os.path.join(GOLDEN, "tiny-q4km.gguf")
+    m = open_model(path, hip_lib, monkeypatch, contexts=2, ctx=128)
+    alone = open_model(path, hip_lib, monkeypatch, ctx=128)
+    lib = m._lib
+    lib.ctamd_profile_decode.restype, lib.ctamd_profile_decode.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int]
+    lib.ctamd_trace_site.restype, lib.ctamd_trace_site.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_int]
+    buf, stamps = (LaunchStat * 32)(), (ctypes.c_uint64 * 512)()
+    toks = [int(t) for t in np.random.default_rng(4).integers(3, m.vocab_size, 24)]
+    for h in (m, alone):
+        h.eval(toks[:20])
+    if active == 1:
+        m.use_context(1)
+        m.eval(toks[20:21])                  # (its position 0 becomes context 0's)
+    m.fork_context(0, 1)
+    assert lib.ctamd_profile_decode(m._llm, 2, buf, 32) <= 0 and lib.ctamd_trace_site(m._llm, b"qkv", stamps, 8) < 0
+    m.use_context(0)
+    got = logits_after(m, toks[21:22], toks[22:23])
+    assert np.array_equal(got, logits_after(alone, toks[21:22], toks[22:23]))
+    assert lib.ctamd_profile_decode(m._llm, 1, buf, 32) > 0              # an eval's last token is there again
+    m.free_context(0)
+    assert lib.ctamd_profile_decode(m._llm, 1, buf, 32) <= 0
