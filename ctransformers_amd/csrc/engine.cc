@@ -1442,7 +1442,11 @@ bool Engine::decode_burst(int n, double* us_per_token, std::string& err) {
     if (last_pos_ + 1 + n >= n_ctx_ || n < 1 || n > 100) { err = "decode_burst: would run past the context"; return false; }
     if (!drain_spec(err)) return false;
     if (!ensure_graphs(err)) return false;
-    if (kv4_ && !kv4_room(last_pos_ + 1, n, err)) return false;
+    if (kv4_) {
+        const int len = ctxs_[active_].len;   // (what the burst writes is no part of the context)
+        if (!kv4_room(last_pos_ + 1, n, err)) return false;
+        ctxs_[active_].len = len;
+    }
     // the cursor as the next eval would set it; the token ids are whatever the last request left in d_tokens_ (timing only) — with
     // continuation graphs the burst IS the greedy chain (each head launch hands the next step its token)
     h_scalars_[0] = 0; h_scalars_[1] = last_pos_ + 1; h_scalars_[2] = last_pos_ + 1 + (graph_cont_[0] ? 1 : n); h_scalars_[3] = 0;

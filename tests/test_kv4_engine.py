@@ -263,3 +263,20 @@ def test_measurements_do_not_write_into_pages_that_a_fork_shares(hip_lib, active
     assert lib.ctamd_profile_decode(m._llm, 1, buf, 32) > 0              # an eval's last token is there again
     m.free_context(0)
     assert lib.ctamd_profile_decode(m._llm, 1, buf, 32) <= 0
+
+
+@pytest.mark.gpu
+def test_a_burst_is_no_part_of_the_context(hip_lib, monkeypatch):
+    path = os.path.join(GOLDEN, "tiny-q4km.gguf")
+    m = open_model(path, hip_lib, monkeypatch, contexts=2, ctx=256)
+    alone = open_model(path, hip_lib, monkeypatch, ctx=256)
+    m._lib.ctamd_decode_burst.restype, m._lib.ctamd_decode_burst.argtypes = ctypes.c_double, [ctypes.c_void_p, ctypes.c_int]
+    toks = [int(t) for t in np.random.default_rng(5).integers(3, m.vocab_size, 70)]
+    for h in (m, alone):
+        h.eval(toks[:60])
+    assert m._lib.ctamd_decode_burst(m._llm, 100) > 0                     # (through two pages' ends)
+    assert m._extension("ctamd_context_length", 0) == 60
+    m.fork_context(0, 1)
+    assert m._extension("ctamd_context_length", 1) == 60 and m.compact_contexts() == 3   # what the burst has taken stays the first context's until it is written over
+    m.use_context(1)
+    assert np.array_equal(logits_after(m, toks[60:61], toks[61:62]), logits_after(alone, toks[60:61], toks[61:62]))
