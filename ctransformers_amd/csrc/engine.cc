@@ -400,8 +400,8 @@ void Engine::debug_dump(const char* site, int layer) {
     if (!strcmp(site, "2attn")) {  // also the layer's K/V cache
         const int G = hp_.n_embd_gqa();
         std::vector<uint16_t> kv((size_t)n_ctx_ * G + (size_t)v_stride_ * G);
-        (void)hipMemcpy(kv.data(), kcache_ + (size_t)layer * n_ctx_ * G, (size_t)n_ctx_ * G * 2, hipMemcpyDeviceToHost);
-        (void)hipMemcpy(kv.data() + (size_t)n_ctx_ * G, vcache_ + (size_t)layer * v_stride_ * G, (size_t)v_stride_ * G * 2, hipMemcpyDeviceToHost);
+        (void)hipMemcpy(kv.data(), kcache_ + (size_t)layer * kc_layer_, (size_t)n_ctx_ * G * 2, hipMemcpyDeviceToHost);
+        (void)hipMemcpy(kv.data() + (size_t)n_ctx_ * G, vcache_ + (size_t)layer * vc_layer_, (size_t)v_stride_ * G * 2, hipMemcpyDeviceToHost);
         snprintf(name, sizeof(name), "%s/t%04d_l%02d_kv.bin", dump_dir_, dump_seq_, layer);
         f = fopen(name, "wb");
         if (f) { fwrite(kv.data(), 2, kv.size(), f); fclose(f); }

@@ -280,3 +280,25 @@ def test_a_burst_is_no_part_of_the_context(hip_lib, monkeypatch):
     assert m._extension("ctamd_context_length", 1) == 60 and m.compact_contexts() == 3   # what the burst has taken stays the first context's until it is written over
     m.use_context(1)
     assert np.array_equal(logits_after(m, toks[60:61], toks[61:62]), logits_after(alone, toks[60:61], toks[61:62]))
+
+
+def test_the_dump_of_a_handle_with_one_layers_rows(lib, tmp_path, monkeypatch):
+    """CT_AMD_DUMP writes a layer's K / V rows after its attention: with the 4-bit cache they lie in one layer's buffer, which all layers use in turn"""
+    if lib == HIP_LIB:
+        pytest.skip("the emulation alone: the copy is the host's")
+    path = os.path.join(GOLDEN, "tiny-q4km.gguf")
+    rows = {}
+    for kv in ("f16", "q4"):
+        out = tmp_path / kv
+        out.mkdir()
+        m = open_model(path, lib, monkeypatch, kv=kv, ctx=32, CT_AMD_DUMP=out)
+        m.eval([5])
+        for il in (0, 1):
+            name = sorted(f for f in os.listdir(out) if f.endswith("_l%02d_kv.bin" % il))[-1]
+            rows[kv, il] = np.fromfile(out / name, np.float16).astype(np.float32)
+        del m
+    monkeypatch.delenv("CT_AMD_DUMP")
+    assert np.array_equal(rows["f16", 0], rows["q4", 0])
+    a, b = rows["f16", 1], rows["q4", 1]
+    assert a.any() and np.array_equal(a != 0, b != 0)                     # one position's rows, and zeros everywhere else
+    assert np.linalg.norm(a - b) < 0.3 * np.linalg.norm(a)                 # layer 0 attended to V in 4 bits: half a step of 1/8 of a group's largest, 1/16, at worst in every value
