@@ -516,6 +516,9 @@ template <int G> DEV int kv4_dim(int j, int i, int r) {
 
 template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 : G * NT <= 4 ? 3 : 2) kv4_decode_kernel(const Kv4Attn a) {
     constexpr int W = 4, DP = 32 * G, PITCH = DP + 4, ROWS = 16 * NT;
+    // -8 sum(q) is the K product's C operand, four registers of one value; two tiles of 128 dims have no room for them (20 registers were spilled) and add it afterwards.
+    // us for 12, 24, 48 rows a KV head behind 4000 tokens, 16 sequences: 42 / 38, 46 / 42, 48 / 45 added afterwards; with one tile 66 / 68 (64 sequences).
+    constexpr bool LATE = G == 4 && NT == 2;
     CT_DYN_SMEM(smem);
     float* part = (float*)smem;                       // [wave][row][PITCH] of one row tile
     float* stat = part + W * 16 * PITCH;              // [wave][ROWS][2]: maximum, sum
@@ -563,7 +566,8 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
     const bool whole = begin == 0 && end == nb;
 
     u32x4 q[NT][G];
-    f32x4 cq[NT][G];
+    f32x4 cq[LATE ? 1 : NT][LATE ? 1 : G];
+    float cl[LATE ? NT : 1][LATE ? G : 1];
     float sc2[NT], mx[NT], sum[NT];
     int lim[NT];
     f32x4 O[NT][2 * G];
@@ -576,8 +580,11 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
         const long long at = (long long)(lo + tok) * a.q.row + (long long)(kvh * a.rep + (on ? r - tok * a.rep : 0)) * a.q.head;
         const float down = kv4_query<G>(q[n], a.q, at, 8 * i, 32, c.head_dim, on, a.scale, [](float v) { v = fmaxf(v, lane_xor16(v)); return fmaxf(v, lane_xor32(v)); });
 #pragma unroll
-        for (int g = 0; g < G; ++g)   // -8 sum(Q) of the group in every row of the product: A all -8 (f16 bits 0x8008: -8 * 2^-24, as the codes are)
-            cq[n][g] = mfma_f16_16x16x32(u32x4_of(0x80088008u, 0x80088008u, 0x80088008u, 0x80088008u), q[n][g], f32x4_splat(0.0f));
+        for (int g = 0; g < G; ++g) {   // -8 sum(Q) of the group in every row of the product: A all -8 (f16 bits 0x8008: -8 * 2^-24, as the codes are)
+            const f32x4 c8 = mfma_f16_16x16x32(u32x4_of(0x80088008u, 0x80088008u, 0x80088008u, 0x80088008u), q[n][g], f32x4_splat(0.0f));
+            if constexpr (LATE) cl[n][g] = c8[0];
+            else cq[n][g] = c8;
+        }
         sc2[n] = kv4_factor(a.scale, down, 16777216.0f);
         mx[n] = -INFINITY;
         sum[n] = 0.0f;
@@ -617,12 +624,15 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
                     const u32x4 kf = u32x4_of(k & M, (k >> 4) & M, (k >> 8) & M, (k >> 12) & M);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const f32x4 acc = mfma_f16_16x16x32(kf, q[n][g], cq[n][g]);
+                        f32x4 acc;
+                        if constexpr (LATE) acc = mfma_f16_16x16x32(kf, q[n][g], f32x4_splat(0.0f));
+                        else acc = mfma_f16_16x16x32(kf, q[n][g], cq[n][g]);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const uint32_t d2 = ks[t][2 * g + e / 2];
                             const float d = f16_bits_to_f32((uint16_t)(e & 1 ? d2 >> 16 : d2 & 0xFFFFu));
-                            s[n][t][e] = g == 0 ? d * acc[e] : fmaf(d, acc[e], s[n][t][e]);
+                            const float x = LATE ? acc[e] + cl[LATE ? n : 0][LATE ? g : 0] : acc[e];
+                            s[n][t][e] = g == 0 ? d * x : fmaf(d, x, s[n][t][e]);
                         }
                     }
                 }

@@ -31,3 +31,12 @@ def test_product_build_has_no_register_spills():
     # vector-register spills and scratch memory are what costs; scalar registers parked in vector lanes (v_writelane) touch no memory
     bad = {k: v for k, v in kernels.items() if v.get("VGPRs Spill", 0) or v.get("ScratchSize [bytes/lane]", 0)}
     assert not bad, "kernels with vector-register spills / scratch memory: %s" % bad
+
+
+@pytest.mark.skipif(not os.path.exists(LOG), reason="the library has not been built here")
+def test_the_log_holds_the_kernels_of_every_translation_unit():
+    """what the check above reads: the operators' kernels are compiled on their own, and stand there too"""
+    names = re.findall(r"remark: Function Name: (\S+)", open(LOG).read())
+    for kernel, count in (("kv4_decode_kernel", 10), ("kv4_prompt_kernel", 6), ("kv4_join_kernel", 8), ("kv4_append_kernel", 6), ("kv4_read_kernel", 6),
+                          ("kv_reserve_plan_kernel", 1), ("kv_compact_apply_kernel", 1), ("matvec_v9", 1), ("attn_fused", 1)):
+        assert len({n for n in names if kernel in n}) >= count, kernel
