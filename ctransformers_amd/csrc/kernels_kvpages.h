@@ -15,6 +15,14 @@ static inline void kvp_atomic_add(int* p, int v) { *p += v; }
 #else
 DEV void kvp_atomic_add(int* p, int v) { (void)atomicAdd(p, v); }
 #endif
+// words that threads of one workgroup count in: read and cleared where atomics are performed
+#ifdef CT_EMU
+static inline int kvp_atomic_get(int* p) { return *p; }
+static inline void kvp_atomic_clear(int* p) { *p = 0; }
+#else
+DEV int kvp_atomic_get(int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+DEV void kvp_atomic_clear(int* p) { __hip_atomic_store(p, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+#endif
 
 // exclusive sum over the workgroup's threads; `all` = the total
 DEV int kvp_scan(int v, int& all, int* lds) {
@@ -89,11 +97,11 @@ __global__ void __launch_bounds__(256) kv_fork_counts_kernel(const KvPages a) {
 
 // ---- reserve: room for add[s] more tokens in every sequence -----------------------------------------------------------------------------------------
 // ws: [0] ok, [1] copies, [2] pages taken, [4 ..] per sequence {first entry that changes, entries, index of its first page among those taken, copied tail or -1},
-// then the pages taken, then the copies (source, destination)
-struct KvpWs { int* head; int* seq; int* taken; int* copy; };
+// then the pages taken, then the copies (source, destination), then per page how many of the rounds' sequences had it as their partly filled last page
+struct KvpWs { int* head; int* seq; int* taken; int* copy; int* sharers; };
 DEV KvpWs kvp_ws(const KvPages& a) {
     KvpWs w;
-    w.head = a.ws; w.seq = a.ws + 4; w.taken = w.seq + 4 * (long long)a.n_seq; w.copy = w.taken + a.n_pages;
+    w.head = a.ws; w.seq = a.ws + 4; w.taken = w.seq + 4 * (long long)a.n_seq; w.copy = w.taken + a.n_pages; w.sharers = w.copy + 2 * (long long)a.n_seq;
     return w;
 }
 __global__ void __launch_bounds__(kPlanThreads) kv_reserve_plan_kernel(const KvPages a) {
@@ -108,6 +116,13 @@ __global__ void __launch_bounds__(kPlanThreads) kv_reserve_plan_kernel(const KvP
     }
     const KvpWs w = kvp_ws(a);
     if (tid == 0) flags = 0;
+    const bool rounds = a.n_seq > kPlanThreads;   // a sequence of the first round finds those before it in LDS, one of a later round needs the counts too
+    if (rounds) {
+        for (int p = tid; p < a.n_pages; p += kPlanThreads) kvp_atomic_clear(&w.sharers[p]);
+#ifndef CT_EMU
+        __threadfence();
+#endif
+    }
     __syncthreads();
     int taken = 0, copies = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += kPlanThreads) {
@@ -127,31 +142,27 @@ __global__ void __launch_bounds__(kPlanThreads) kv_reserve_plan_kernel(const KvP
                 const int p = a.table[(long long)s * a.width + first];
                 if (p >= 0 && p < a.n_pages) tail = p;
             }
-            w.seq[4 * (long long)s + 3] = tail;      // (for the threads of later rounds)
         }
         __syncthreads();
         tails[tid] = tail;
         __syncthreads();
         bool copied = false;
         if (tail >= 0 && a.refs[tail] > 1) {         // shared: those that come before take their references away first
-            int left = a.refs[tail];
+            int left = a.refs[tail] - (s0 ? kvp_atomic_get(&w.sharers[tail]) : 0);
             for (int k = 0; k < tid; ++k) left -= tails[k] == tail;
-            for (int k = 0; k < s0; ++k) {
-                const int t = w.seq[4 * (long long)k + 3];
-                left -= (t >= 0 ? t : -2 - t) == tail;   // (-2 - t: a tail that was not copied, see below)
-            }
             copied = left > 1;
         }
         if (more) {
             start = first + (partly && tail >= 0 && !copied);
             need = last - start < a.width ? (int)(last - start) : a.width;   // (more than that is refused below)
         }
-        __syncthreads();                             // every thread has read the earlier rounds' tails
+        __syncthreads();                             // every thread has read the earlier rounds' counts
+        if (rounds && tail >= 0) kvp_atomic_add(&w.sharers[tail], 1);
         int all, c_all;
         const int at = kvp_scan(need, all, lds), c_at = kvp_scan(copied ? 1 : 0, c_all, lds);
         if (s < a.n_seq) {
             int* q = w.seq + 4 * (long long)s;
-            q[0] = start; q[1] = need; q[2] = taken + at; q[3] = copied ? tail : tail >= 0 ? -2 - tail : -1;
+            q[0] = start; q[1] = need; q[2] = taken + at; q[3] = copied ? tail : -1;
             if (copied) { w.copy[2 * (copies + c_at)] = tail; w.copy[2 * (copies + c_at) + 1] = taken + at; }   // (an index among the taken pages, for now)
         }
         if (all > 0x3FFFFFFF - taken) all = 0x3FFFFFFF - taken;   // (saturates: more pages than there can be)

@@ -379,7 +379,7 @@ int ctamd_kv_fork(const ctamd_kv_tables* t, const int* parents, const int* keep,
     const bool ok = ctamd::kv_fork(a, (hipStream_t)stream, err);   // (before err is read)
     return ops_result(ok, "kv_fork", err);
 }
-long long ctamd_kv_reserve_ws(int n_seq, int n_pages) { return 4 + 6ll * n_seq + n_pages; }
+long long ctamd_kv_reserve_ws(int n_seq, int n_pages) { return 4 + 6ll * n_seq + 2ll * n_pages; }
 int ctamd_kv_reserve(const ctamd_kv_tables* t, const int* add, void* pages, int layers, long long layer_stride, long long page_bytes, int* status, int* ws,
                      void* stream) {
     const char* err = "null tables";

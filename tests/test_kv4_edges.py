@@ -1,6 +1,7 @@
 """The 4-bit paged KV cache (ctransformers_amd/ops.py, csrc/engine_kv4.h) at the edges of what its calls accept."""
 import ctypes
 import math
+import time
 
 import numpy as np
 import pytest
@@ -265,3 +266,30 @@ def test_no_length_beyond_2_31(dev):
         t, n, r, short = ops.kv_reserve(pages, table, lens, refs, ints(dev, add), page_tokens=2**30)
         assert int(short) == want and n.tolist() == [length + (0 if want else add)]
         assert torch.equal(t, table) and torch.equal(r, refs)
+
+
+def shared_by_all(dev, n):
+    """n sequences of five tokens in two pages of four, forks of one another; room for one more each"""
+    table = torch.tensor([[0, 1, -1]], dtype=torch.int32).repeat(n, 1).to(dev)
+    refs = torch.zeros(n + 1, dtype=torch.int32, device=dev)
+    refs[:2] = n
+    pages = torch.zeros((n + 1, 16), dtype=torch.uint8, device=dev)
+    lens, add = torch.full((n,), 5, dtype=torch.int32, device=dev), torch.ones(n, dtype=torch.int32, device=dev)
+    t0 = time.perf_counter()
+    t, m, r, short = ops.kv_reserve(pages, table, lens, refs, add, page_tokens=4)
+    assert int(short) == 0
+    took = time.perf_counter() - t0
+    # pages 2, 3, .. in order; the last sequence keeps the shared one
+    assert t[:, 0].tolist() == [0] * n and t[:, 1].tolist() == list(range(2, n + 1)) + [1] and m.tolist() == [6] * n
+    assert r.tolist() == [n] + [1] * n
+    return took
+
+
+def test_room_for_very_many_sequences_of_one_last_page(dev):
+    """in time that grows with their number, not with its square"""
+    shared_by_all(dev, 3000)
+    if dev.type == "cuda":
+        assert shared_by_all(dev, 1 << 20) < 1.0
+        return
+    few, many = (min(shared_by_all(dev, n) for _ in range(2)) for n in (1 << 15, 1 << 17))
+    assert many < 5 * few   # (linear: less than 4; quadratic: towards 16)
