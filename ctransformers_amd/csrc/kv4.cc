@@ -260,8 +260,8 @@ bool kv_fork(const KvPages& a, hipStream_t stream, const char*& err) {
     if (a.n_new && !a.parents) { err = "null parents"; return false; }
     const long long cells = (long long)a.n_new * a.width;
     if (!queue(err, kv_fork_rows_kernel, dim3(groups_for(cells > a.n_pages ? cells : a.n_pages, 256, 2048)), dim3(256), 0, stream, a)) return false;
-    const int rows = a.n_seq + (a.keep ? a.n_new : 0);
-    return !rows || queue(err, kv_fork_counts_kernel, dim3((unsigned)rows), dim3(256), 0, stream, a);
+    const int each = a.keep || a.n_new > kForkEach, rows = a.n_seq + (each ? a.n_new : 0);
+    return !rows || queue(err, kv_fork_counts_kernel, dim3((unsigned)rows), dim3(256), 0, stream, a, each);
 }
 bool kv_reserve(const KvPages& a, hipStream_t stream, const char*& err) {
     if (!pages_check(a, true, err) || !move_check(a, err)) return false;

@@ -293,3 +293,23 @@ def test_room_for_very_many_sequences_of_one_last_page(dev):
         return
     few, many = (min(shared_by_all(dev, n) for _ in range(2)) for n in (1 << 15, 1 << 17))
     assert many < 5 * few   # (linear: less than 4; quadratic: towards 16)
+
+
+@pytest.mark.parametrize("n_new", [4096, 4097])
+def test_forks_into_very_many(dev, n_new):
+    """either way of counting references: parents with many children, one, and none, children of nobody"""
+    n, width = 40, 3
+    g = torch.Generator().manual_seed(n_new)
+    table = torch.randperm(n * width, generator=g)[:n * width].view(n, width).int()
+    lens = torch.randint(0, 4 * width + 1, (n,), generator=g).int()
+    used = (lens[:, None] + 3) // 4 > torch.arange(width)
+    table[~used] = -1
+    refs = torch.zeros(n * width + 1, dtype=torch.int32)
+    refs[table[used].long()] = 1
+    parents = torch.cat([torch.tensor([n, -1, 3, 5]), torch.randint(6, n, (n_new - 4,), generator=g)]).int()
+    t, m, r = (x.cpu() for x in ops.kv_fork(table.to(dev), lens.to(dev), refs.to(dev), parents.to(dev), page_tokens=4))
+    ok = (parents >= 0) & (parents < n)
+    at = parents.clamp(0, n - 1).long()
+    want = torch.where(ok[:, None], table[at], -1)
+    counts = torch.zeros_like(refs).index_add_(0, want[want >= 0].long(), torch.ones(int((want >= 0).sum()), dtype=torch.int32))
+    assert torch.equal(t, want) and torch.equal(m, torch.where(ok, lens[at], 0)) and torch.equal(r, counts)
