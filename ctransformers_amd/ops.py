@@ -14,7 +14,8 @@ tensors on the device; a table entry outside [0, n_pages) names no page (rows fo
 
 Every operator runs on the current stream of its tensors' device and returns without waiting for it; nothing is kept between calls.  Workspaces and results come from
 torch's allocator, so calls can be captured into a graph and several graphs share nothing.  What a user may get wrong raises ValueError / TypeError before anything is
-launched.  There is no CPU path: without the HIP library, or with tensors elsewhere than on a GPU, a call raises.  No operator has a gradient.
+launched.  There is no CPU path: without the HIP library, or with tensors elsewhere than on a GPU, a call raises.  No operator has a gradient:
+q, k, v or out that require one are refused unless gradients are off.
 """
 import ctypes
 import math
@@ -105,6 +106,8 @@ def _rows(device, name, x, shape=None):
         raise TypeError("%s is a float16, bfloat16 or float32 tensor" % name)
     if x.get_device() != device:
         raise ValueError("%s is on %s, not on device %d" % (name, x.device, device))
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires a gradient, and no operator has one: detach it, or call under torch.no_grad()" % name)
     if len(x.shape) != 3 or (shape is not None and x.shape != shape):
         raise ValueError("%s has shape %s%s" % (name, tuple(x.shape), "" if shape is None else ", not %s" % (tuple(shape),)))
     return ROWS.pack(x.data_ptr(), *x.stride(), t)

@@ -246,6 +246,26 @@ def test_an_error_that_another_call_left(dev):
     assert (out == 1).all()
 
 
+def test_a_gradient_is_not_lost_in_silence(dev):
+    c = Cache(1, [40], 1, 32, 32)
+    c.fill(2)
+    pages, table, lens = c.on(dev)
+    old = pages.clone()
+    x = torch.ones((1, 1, 32), device=dev)
+    g = torch.ones((1, 1, 32), device=dev, requires_grad=True)
+    att = lambda q, out=None: ops.kv4_attention(q, pages, table, lens, None, 1, n_head_kv=1, page_tokens=32, out=out)  # noqa: E731
+    app = lambda k, v: ops.kv4_append(k, v, pages, table, lens, None, 1, page_tokens=32)  # noqa: E731
+    for call in (lambda: att(g), lambda: att(x, g), lambda: att(g * 2), lambda: app(g, x), lambda: app(x, g)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    assert torch.equal(pages, old)
+    want = att(x)
+    assert torch.equal(att(g.detach()), want)
+    with torch.no_grad():
+        assert torch.equal(att(g), want)
+        app(g, x)
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("length,add", [(2**31 - 1, 2**31 - 1), (1, 2**31 - 1), (2**31 - 1, 1), (2**30, 2**30)])
 def test_room_behind_lengths_near_2_31(dev, length, add):
