@@ -333,3 +333,42 @@ def test_forks_into_very_many(dev, n_new):
     want = torch.where(ok[:, None], table[at], -1)
     counts = torch.zeros_like(refs).index_add_(0, want[want >= 0].long(), torch.ones(int((want >= 0).sum()), dtype=torch.int32))
     assert torch.equal(t, want) and torch.equal(m, torch.where(ok, lens[at], 0)) and torch.equal(r, counts)
+
+
+# ---- graphs ---------------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [96, 128, 256])
+@pytest.mark.parametrize("news", [1, 6, 150])
+def test_every_attention_kernel_in_a_graph(hip_lib, dim, news):
+    """head sizes whose kernels take more LDS than a launch may without asking, the asking within the capture: replays equal eager calls, with eager work between them"""
+    ops.load(hip_lib)
+    dev = torch.device("cuda:0")  # noqa: F811
+    heads, H, page, B, width = 2, 8, 64, 2, 24
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        lens = torch.randint(news, width * page + 1, (B,), generator=g).int()
+        pages = torch.zeros((B * width, ops.kv4_page_bytes(heads, dim, page)), dtype=torch.uint8, device=dev)
+        table = torch.randperm(B * width, generator=g).view(B, width).int().to(dev)
+        total = int(lens.sum())
+        k, v = (torch.randn((total, heads, dim), generator=g).half().to(dev) for _ in range(2))
+        ops.kv4_append(k, v, pages, table, lens.to(dev), ints(dev, 0, int(lens[0]), total), int(lens.max()), page_tokens=page)
+        return [torch.randn((B * news, H, dim), generator=g).half().to(dev), pages, table, lens.to(dev)]
+
+    cu = ints(dev, 0, news, 2 * news)
+    run = lambda x: ops.kv4_attention(*x, cu, news, n_head_kv=heads, page_tokens=page)  # noqa: E731
+    held = inputs(0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(held)
+    for seed in range(1, 5):
+        new = inputs(seed)
+        for x, y in zip(held, new):
+            x.copy_(y)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, run(new))
+        graph.replay()
+        assert torch.equal(out, got)
