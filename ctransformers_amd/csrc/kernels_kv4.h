@@ -42,7 +42,6 @@ static inline u32x4 u32x4_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { r
 static inline f32x4 f32x4_splat(float x) { return f32x4{{x, x, x, x}}; }
 static inline uint32_t bits_of(float f) { uint32_t u; memcpy(&u, &f, 4); return u; }
 static inline float float_of(uint32_t u) { float f; memcpy(&f, &u, 4); return f; }
-static inline void atomic_add_i32(int* p, int v) { *p += v; }
 #else
 typedef _Float16 kv4_h2 __attribute__((ext_vector_type(2)));
 DEV uint32_t kv4_add2(uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(kv4_h2, a) + __builtin_bit_cast(kv4_h2, b)); }
@@ -62,7 +61,6 @@ DEV u32x4 u32x4_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return u32x
 DEV f32x4 f32x4_splat(float x) { return f32x4{x, x, x, x}; }
 DEV uint32_t bits_of(float f) { return __builtin_bit_cast(uint32_t, f); }
 DEV float float_of(uint32_t u) { return __builtin_bit_cast(float, u); }
-DEV void atomic_add_i32(int* p, int v) { (void)atomicAdd(p, v); }
 #endif
 // an index that the compiler has to take as new: what follows from it is computed where it is used and not kept in registers around an outer loop
 #ifdef CT_EMU
@@ -121,7 +119,8 @@ DEV void kv4_load8(float (&x)[8], const Kv4Rows& r, long long at) {
 }
 // A query row's pieces as halves: N pieces of eight dims, piece k at at + 8 * (k * step + lane's), dims from head_dim on are zeros.  Rows that f16 may not hold (bf16,
 // f32) are scaled by a power of two that brings the row's largest value into [1, 2) — all lanes that hold pieces of a row agree on it through `across` — so that bf16
-// stays exact but for values below 2^-17 of the largest.  Returns the inverse of the scale.
+// stays exact but for values below 2^-17 of the largest.  float32 is rounded to f16's 11 bits, 2^-11 of a value: the products that stream the codes at memory speed, and
+// those that keep up with a prompt, take halves; a second half of q would be another product for each of K's.  Returns the inverse of the scale.
 // A negative `scale` goes into the query's sign: scores can then be compared before they are scaled.
 template <int N, class Across> DEV float kv4_query(u32x4 (&q)[N], const Kv4Rows& r, long long at, int d0, int step, int head_dim, bool on, float scale, Across across) {
     const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;
@@ -169,7 +168,7 @@ DEV float kv4_factor(float scale, float down, float unit) { return fminf(fmaxf((
 constexpr float kFar = 0x1p22f;
 // Weights are halves for the matrix instructions.  They are relative to a number that lies kRaise below the row's running maximum and is moved only when a score passes that
 // maximum by more than kLag: at most 2^15, and what is lost at the small end lies 2^-(24 + kRaise) below the maximum instead of 2^-24 (a long flat tail counts).
-constexpr float kRaise = 11.0f, kLag = 15.0f - kRaise;   // (times of all sizes: the same with 7, 9 and 11; with 14 maxima move often, prompts take 5 % longer)
+constexpr float kRaise = 11.0f, kLag = 15.0f - kRaise;   // (a prompt of 2048 tokens, us: 71.2 with 7, 71.4 with 9, 72.1 with 11; with 14 maxima move often, 5 % more; token steps the same)
 // eight neighbouring dims out; vec: as for loads
 DEV void kv4_store8(void* p, long long at, int type, int vec, const float (&x)[8]) {
     if (vec && type != KV4_F32) {
@@ -228,7 +227,7 @@ DEV const uint8_t* kv4_in_page(const Kv4Cache& c, int pid, int h, int blk) {
 // One workgroup per (block, head) that new rows fall into: it alone writes that block, so a V dword that keeps older tokens is read, changed and written without
 // atomics.  A lane takes eight dims (16 bytes of a half row, so that a wave reads whole lines), four lanes a group; they agree on the largest value by two quad
 // exchanges.  K codes and scales go straight out, V codes cross the workgroup through LDS (eight tokens to a dword).  All loads of a lane are issued before the
-// first value is used.  16 prompts of up to 1500 tokens, 64 heads of 112 in float32 (585 MB in, 101 MB out): 217 us, 3.2 TB/s; one token of 64 sequences, 8 heads:
+// first value is used.  16 prompts of up to 1500 tokens, 64 heads of 112 in float32 (702 MB in, 113 MB out): 216 us, 3.8 TB/s; one token of 64 sequences, 8 heads:
 // 6.4 us, latency (cursor -> table -> rows -> codes -> store).
 template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
     __shared__ uint32_t vcode[32][8 * G + 1];   // V codes as bytes [token][dim]; + 1: tokens in different banks
@@ -335,7 +334,7 @@ template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const 
 }
 
 // The last rows of every sequence out of the cache, as numbers: the mirror image of kv4_append_kernel, same workgroups.  Rows whose page is absent are zeros.
-// The same prompts (101 MB in, 292 MB of halves out): 119 us, 3.3 TB/s.
+// The same prompts (113 MB in, 351 MB of halves out): 119 us, 3.9 TB/s.
 template <int G> __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Append a) {
     const Kv4Cache& c = a.c;
     const int tid = (int)threadIdx.x, h = (int)blockIdx.x % c.n_head_kv, place = (int)blockIdx.x / c.n_head_kv, b = place / a.blocks;   // (heads lie side by side in a row)
@@ -483,10 +482,11 @@ DEV u32x4 kv4_values(uint32_t w, uint32_t s0, uint32_t s1, uint32_t s2, uint32_t
 // multiplies the 32-dim product in f32, so K is used exactly.  Maximum, sum and O stay per lane in f32; the maximum is raised (and O rescaled) only when a score
 // passes it by more than 2^kLag, so most blocks exchange nothing between lanes.  P enters as two halves, the rounded one and what it left (the matrix cores have the time:
 // +2 % at most): off by 2^-22 of p, or 2^-36 of the row's largest where p is smaller than that allows.  V's product with its scale is one half, 2^-11.
-// Memory-bound: one sequence of 130 000 tokens, 8 KV heads of 128 with 8 query heads each (150 MB): 34 us, 4.4 TB/s; 64 sequences of 0 .. 8192 tokens (306 MB): 70 us,
-// 4.4 TB/s (a large copy moves 4.66).  One sequence of 140 tokens: 7.2 us, latency.
+// One sequence of 130 000 tokens, 8 KV heads of 128 with 8 query heads each (150 MB): 35 us, 4.3 TB/s; 64 sequences of 0 .. 8192 tokens (303 MB): 71 us, 4.3 TB/s.  A large
+// copy moves 4.66 TB/s, reading alone reaches 6.4 .. 6.6: memory is not all of it.  Counters of the second: vector units 54 % busy, matrix cores 14 %, 2.1 waves a SIMD,
+// which wait for data 30 % and for their turn to issue 36 % of their time.  One sequence of 140 tokens: 7.3 us, latency.
 // The next block's K is fetched into the registers of this one's as soon as its scores are there, its V after the V product: 40 dwords a lane at 128 dims for a
-// block in flight, which leaves room for four waves a SIMD.
+// block in flight, which leaves room for three waves a SIMD (146 registers).
 template <int G> DEV void kv4_fetch_k(uint32_t (&kc)[2][G], uint32_t (&ks)[2][2 * G], const uint8_t* blk, int m, int i) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -848,9 +848,10 @@ template <int NR, bool LINE, int W> __global__ void __launch_bounds__(64 * W) kv
 // The row tiles of one (sequence, KV head) go to one XCD, whose L2 then holds that head's codes for all of them; tiles that see most come first.
 // Rounded on the way: K's and V's values and p to halves (2^-11 each at most, p below 2^-25 of the row's largest by up to 2^-36 of that; the 32 x 32 products want halves).  A float16 result is off by 3.8e-4 of its norm, its own
 // rounding alone by 2.1e-4; K exact, as in the kernel above, would take 128 more fused multiply-adds and 32 more LDS reads a step.
-// 2048 tokens, 32 heads of 128 (34 GFLOP): 79 us, 437 TFLOP/s; 4 chunks of up to 512 behind up to 8000 tokens, 64 / 8 heads (234 GFLOP): 372 us, 630 TFLOP/s (a large
-// f16 product: 1142).  Bound by the vector units: 270 instructions a step and wave (exp2 a quarter of their time) take 1300 cycles beside 1024 of matrix products, two
-// waves a SIMD overlap them in part; 33 % of the waves' time is waits.  Measured and not taken: one block a step and three waves a SIMD (96 / 421 us), unpacking
+// 2048 tokens, 32 heads of 128 (34 GFLOP): 72 - 81 us, 424 - 477 TFLOP/s; 4 chunks of up to 512 behind up to 8000 tokens, 64 / 8 heads (252 GFLOP): 333 - 391 us, 645 - 758
+// TFLOP/s (a large f16 product: 1142).  Neither pipe is full: counters of the chunks have the vector units 41 % busy and the matrix cores 31 %, with 1.6 waves a SIMD of the two
+// that fit, which wait 33 % of their time (the prompt: 26 %, 18 %, 1.2 waves, 35 %).  What is lost is overlap — 270 vector instructions a step and wave beside 1024 cycles of
+// matrix products — and the ends of launches, where the longest tiles run alone.  Measured and not taken: one block a step and three waves a SIMD (96 / 421 us), unpacking
 // between the K.Q products (82 / 371), wave priorities around them (no change), all pairs' long tiles first (chunks 635).
 template <int G> struct Kv4Lds { static constexpr int KC = 32 * 16 + 32, KB = 4 * G * KC, VB = 4 * 32 * G * 16, BLK = KB + VB, BYTES = 4 * BLK; };
 

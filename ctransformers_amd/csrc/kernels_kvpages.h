@@ -2,9 +2,10 @@
 // lives in device memory — tables of page numbers, lengths, one count of references per page (0: free) — so that no operation waits for the host and all of them can be
 // captured into a graph.  Everything is deterministic: free pages are taken lowest first, in the order of the sequences.
 //
-// reserve and compact are two launches each: workgroup 0 of the first plans (a scan over the sequences and the pages: latency, ~1 us per 4096 pages) while the others
-// copy the tables; the second applies the plan and moves the pages, which is a plain copy and bound by memory.  Moving 424 MB (half of a pool of 16 layers): 187 us,
-// 4.5 TB/s read and written (a large copy: 4.66).  256 sequences of up to 8192 tokens: fork 3.0 + 3.2 us, room for 16 more tokens 10.8 + 4.8 us.
+// reserve and compact are two launches each: workgroup 0 of the first plans (a scan over the sequences and the pages: latency, ~1 us per 4096 pages and per 1024 sequences,
+// more where many of those share their last page: each counts those before it among its 1024) while the others copy the tables; the second applies the plan and moves the
+// pages, which is a plain copy and bound by memory.  Moving 424 MB (half of a pool of 16 layers): 190 us, 4.5 TB/s read and written (a large copy: 4.66).  256 sequences of
+// up to 8192 tokens: fork 2.9 + 2.9 us, room for 16 more tokens 11.1 + 4.6 us.
 #pragma once
 #include "kv4.h"
 

@@ -110,9 +110,11 @@ bool kv4_read(Kv4Append& a, int max_rows, hipStream_t stream, const char*& err) 
 }
 
 // Rows of a tile: kv4_decode_kernel takes 16, or 32 where two tiles of a head fit the registers (128 dims), kv4_prompt_kernel 128.  The first streams the codes at
-// memory speed once per tile, the second unpacks them once for 128 rows but takes at least as long for fewer.  Measured, 16 sequences of up to 8000 tokens, 8 KV heads,
-// the first against the second, us: 128 dims 40 rows 42 / 77, 64 rows 50 / 80, 96 rows 63 / 83, 128 rows 82 / 91 (one sequence: 35 / 31, 400 tokens: 34 / 25);
-// 64 dims 64 rows 30 / 52, 96 rows 35 / 55, 128 rows 42 / 56, 256 rows 71 / 102.
+// memory speed once per tile, the second unpacks them once for 128 rows but takes at least as long for fewer.  Where they cross
+// depends on how much work there is in all; the rule looks at the rows of a KV head alone.  The first against the second, us, 16 sequences of 2650 .. 7950 tokens, 8 KV heads:
+// 128 dims 40 rows 77 / 82, 64 rows 83 / 87, 96 rows 110 / 96, 128 rows 140 / 107; 64 dims 64 rows 55 / 62, 96 rows 74 / 68, 128 rows 89 / 74, 192 rows 125 / 118, 256 rows
+// 158 / 128.  One sequence, 128 dims, 128 rows: of 8000 tokens 37 / 38, of 400 tokens 30 / 24.  4 KV heads, 128 dims: 16 sequences of 2000 .. 6000 tokens 40 rows 43 / 42,
+// 96 rows 57 / 53, one of 4000 24 / 25, 28 / 28.  (The first also keeps K exact and p in two halves.)
 static int tile_rows(const Kv4Attn& a, long long rows) {
     if (rows <= 16) return 16;
     if (a.c.groups <= 4 && rows <= (a.c.groups <= 2 ? 192 : 96)) return 32;

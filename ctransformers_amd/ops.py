@@ -8,8 +8,8 @@ several sequences may share.
     table, lens, refs = kv_fork(table, lens, refs, parents, page_tokens=64)                                       # beams; parent -1 frees a sequence
     table, refs, used = kv_compact(pages, table, refs)                                                            # pages in use to the front
 
-Sequences are packed: rows ``cu[b] .. cu[b + 1] - 1`` of q, k and v are the LAST rows of sequence b, whose length with them is ``lens[b]``; no sequence may
-have more than ``max_rows`` of them (rows beyond are not processed).  ``cu=None``: one sequence, all rows.  table, lens, cu, refs, parents and add are int32
+Sequences are packed: rows ``cu[b] .. cu[b + 1] - 1`` of q, k and v are the LAST rows of sequence b, whose length with them is ``lens[b]``; ``cu`` ascends, and
+no sequence may have more than ``max_rows`` rows (rows beyond are not processed).  ``cu=None``: one sequence, all rows.  table, lens, cu, refs, parents and add are int32
 tensors on the device; a table entry outside [0, n_pages) names no page (rows for it are not stored, its tokens are not attended to).
 
 Every operator runs on the current stream of its tensors' device and returns without waiting for it; nothing is kept between calls.  Workspaces and results come from
@@ -193,7 +193,8 @@ def kv4_attention(q, pages, table, lens, cu, max_rows, *, n_head_kv, page_tokens
     """Causal attention of the rows q [total, n_head, head_dim] over the cache: row i of a sequence with n rows sees the positions 0 .. lens - n + i, query head h
     reads KV head h // (n_head / n_head_kv), scores are q.k * scale (finite; default 1 / sqrt(head_dim)).  A row that sees nothing becomes 0.  q is float16, bfloat16 or
     float32; the result has q's type, or is written into `out` [total, n_head, head_dim] of any of the three, where rows that belong to no sequence are left as they
-    are; `out` may be q itself, but shares no memory with any other tensor of the call, nor any two of its own elements.  Products are taken in float16 (K's codes and V's values; q scaled by a power of two per row, and p), everything else in float32."""
+    are; `out` may be q itself, but shares no memory with any other tensor of the call, nor any two of its own elements.  Products are taken in float16 (K's codes and V's values; q scaled by a power of two per row, so that
+    float32 queries keep 11 bits; and p), everything else in float32.  The same call gives the same bits; a row's last bits may depend on the other rows of the call."""
     device = _device_of("pages", pages)
     qr = _rows(device, "q", q)
     total, n_head, head_dim = q.shape
@@ -267,7 +268,7 @@ def kv_fork(table, lens, refs, parents, *, page_tokens, keep=None):
 
 def kv_reserve(pages, table, lens, refs, add, *, page_tokens):
     """(table, lens, refs, short) with room for add[i] more tokens in sequence i: lens grows by it, pages are taken lowest free first in the order of the sequences,
-    and a last page that others share is copied before its sequence writes it.  pages: [n_pages, ..] or [layers, n_pages, ..], any type.  short (int32, on the
+    and a last page that others share is copied before its sequence writes it.  pages: [n_pages, page] or [layers, n_pages, page], any type.  short (int32, on the
     device): 0, or the pages that were missing, or -1 where a sequence outgrows its row of the table, or 2^31 - 1 tokens; then nothing has changed."""
     device = _device_of("table", table)
     _ints(device, "refs", refs, 1)

@@ -85,11 +85,12 @@ long long ctamd_resident_replays(ctransformers_llm* llm);
 int ctamd_falcon_fold(ctransformers_llm* llm);
 int ctamd_debug_read_kv(ctransformers_llm* llm, int layer, unsigned short* k, unsigned short* v);
 int ctamd_debug_read_attn_out(ctransformers_llm* llm, float* dst, int n_tok);
-/* Contexts.  A handle created with CT_AMD_KV=q4 keeps its KV cache in 4 bits, in pages of 64 tokens, and with CT_AMD_CONTEXTS=n (<= 256) holds n sequences on one set of
- * weights: batch_eval reads and writes the ACTIVE one (0 at first), n_past counts its tokens.  All return 0, or -1 with a message on stderr.
+/* Contexts.  A handle created with CT_AMD_KV=q4 keeps its KV cache in 4 bits, in pages of 64 tokens (CT_AMD_KV_PAGE: 32, 64, 128, 256), and with CT_AMD_CONTEXTS=n
+ * (<= 256) holds n sequences on one set of weights: batch_eval reads and writes the ACTIVE one (0 at first), n_past counts its tokens.  All return 0, or -1 with a
+ * message on stderr.
  *   use      the context that the evals from here on belong to (logits and embeddings stay those of the last eval)
  *   fork     dst (its own content is dropped) becomes a copy of src; nothing is copied but, when one of them writes on, the page that is partly filled
- *   free     drops a context's content
+ *   free     drops a context's content (a fork that the active context takes part in, or its freeing, leaves measurements nothing to replay until the next eval)
  *   length   its tokens, -1: no such context        compact   moves the pages in use to the front of the pool; returns their number
  * ctamd_kv4_launches: attention launches over the 4-bit cache issued by this handle (eager launches and graph captures).  ctamd_debug_read_q: the fp16 query rows of
  * the last layer of the last chunk (n_tok rows) or token step (n_tok = 0); returns n_embd. */

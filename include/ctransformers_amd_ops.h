@@ -10,7 +10,7 @@
  *   table   int32 [n_seq][table_stride]: the first table_width entries of a row name the sequence's pages in order; an entry outside [0, n_pages) names none:
  *           rows for it are not stored, and attention treats its tokens as absent
  *   lens    int32 [n_seq]: tokens of each sequence INCLUDING the rows of this call
- *   cu      int32 [n_seq + 1]: sequence b's rows are the packed rows cu[b] .. cu[b + 1] - 1, its last positions; NULL: one sequence, all rows
+ *   cu      int32 [n_seq + 1], ascending: sequence b's rows are the packed rows cu[b] .. cu[b + 1] - 1, its last positions; NULL: one sequence, all rows
  * max_rows: no sequence has more rows than this (rows beyond it are not processed).  head_dim: a multiple of 8 up to 256; page_tokens: 32, 64, 128 or 256.
  * No two sequences of one append may write the same page (ctamd_kv_reserve sees to that). */
 #ifndef CTRANSFORMERS_AMD_OPS_H_
@@ -44,7 +44,7 @@ int ctamd_kv4_read(const ctamd_kv4_cache* cache, const ctamd_rows* k, const ctam
 /* Causal attention of rows [total][n_head][head_dim] over the cache: row i of a sequence with n rows sees positions 0 .. lens - n + i; a row that sees nothing
  * becomes 0.  n_head is a multiple of n_head_kv, dims of q are adjacent (q.dim == out.dim == 1), scale is finite; out may be q itself, but shares no
  * memory with anything else, and no two of its elements are the same memory.  Rows that belong to no sequence are left as they are.
- * ws: ctamd_kv4_attention_ws() floats (a function of the sizes alone, 0 if none are wanted), 16-byte aligned. */
+ * ws: ctamd_kv4_attention_ws() floats (a function of the sizes and the current device, 0 if none are wanted), 16-byte aligned. */
 long long ctamd_kv4_attention_ws(const ctamd_kv4_cache* cache, int n_head);
 int ctamd_kv4_attention(const ctamd_kv4_cache* cache, int n_head, const ctamd_rows* q, const ctamd_rows* out, float scale, float* ws, long long ws_floats,
                         void* stream);
