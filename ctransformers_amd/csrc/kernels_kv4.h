@@ -239,10 +239,11 @@ template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const 
     kv4_seq(c, b, lo, hi, len);
     const int start = len - (hi - lo);                          // position of the first new row (rows before position 0 are dropped)
     const int blk = (start > 0 ? start : 0) / 32 + place % a.blocks;
-    if (blk * 32 >= len || hi == lo) return;
+    const int stop = hi - lo > a.max_rows ? start + a.max_rows : len;   // behind the last row that is taken
+    if (blk * 32 >= stop || hi == lo) return;
     uint8_t* dst = kv4_block(c, b, h, blk);
     if (!dst) return;
-    const int t_lo = start > blk * 32 ? start - blk * 32 : 0, t_hi = len - blk * 32 < 32 ? len - blk * 32 : 32;   // the new tokens of this block
+    const int t_lo = start > blk * 32 ? start - blk * 32 : 0, t_hi = stop - blk * 32 < 32 ? stop - blk * 32 : 32;   // the new tokens of this block
     if (tid < 32) poison[tid] = 0;
     uint32_t* vd = (uint32_t*)(dst + 512 * G);
     uint32_t old[(G + 1) / 2];   // the V dwords that keep older (or the neighbours of newer) tokens: fetched with the rows, not behind them
@@ -342,9 +343,10 @@ template <int G> __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv
     kv4_seq(c, b, lo, hi, len);
     const int start = len - (hi - lo);
     const int blk = (start >= 0 ? start / 32 : -((31 - start) / 32)) + place % a.blocks;   // rows before position 0 are written too (as zeros)
-    if (blk * 32 >= len || hi == lo) return;
+    const int stop = hi - lo > a.max_rows ? start + a.max_rows : len;
+    if (blk * 32 >= stop || hi == lo) return;
     const uint8_t* src = kv4_block(c, b, h, blk);
-    const int t_lo = start > blk * 32 ? start - blk * 32 : 0, t_hi = len - blk * 32 < 32 ? len - blk * 32 : 32;
+    const int t_lo = start > blk * 32 ? start - blk * 32 : 0, t_hi = stop - blk * 32 < 32 ? stop - blk * 32 : 32;
 #pragma unroll
     for (int k = 0; k < G; ++k) {   // pieces as in kv4_append_kernel
         const int it = tid + 256 * k, half = it / (128 * G), t = (it / (4 * G)) & 31, g = (it / 4) % G, o = it & 3, d0 = 32 * g + 8 * o;
@@ -373,6 +375,7 @@ template <int G> __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv
 // The query rows of a (sequence, KV head) are r = token * rep + head, tiles of them share a workgroup; row r sees the positions below
 // len - rows + token + 1.  The blocks that a tile sees are divided into parts of `per` blocks, one workgroup each, `nsplit` of them at most (the grid); a part is
 // as long as it has to be for all of the call's parts to be about `want_parts`, whatever the sequences' lengths are: they are only known on the device.
+DEV int kv4_rows(const Kv4Attn& a, int nq) { return nq < a.max_rows ? nq : a.max_rows; }   // rows of a sequence that are taken
 struct Kv4Range { int nq, n_rows, first_tok, len, lo, nb, per, parts; };
 DEV int kv4_part(const Kv4Attn& a) {   // every lane of the wave calls it
     if (a.nsplit <= 1) return 1;
@@ -391,7 +394,7 @@ DEV Kv4Range kv4_range(const Kv4Attn& a, int b, int tile, int tile_rows, int par
     kv4_seq(a.c, b, lo, hi, r.len);
     r.lo = lo;
     r.nq = hi - lo;
-    const int row0 = tile * tile_rows, all = r.nq * a.rep;
+    const int row0 = tile * tile_rows, all = kv4_rows(a, r.nq) * a.rep;
     r.n_rows = all - row0 < tile_rows ? all - row0 : tile_rows;
     r.first_tok = row0 / a.rep;
     const int last_tok = (row0 + r.n_rows - 1) / a.rep;
@@ -417,8 +420,7 @@ DEV int kv4_unit_blocks(const Kv4Attn& a, int nq, int len) {   // blocks of each
     return nb < 1 ? 1 : nb > cap ? (cap < 1 ? 1 : cap) : nb;
 }
 DEV int kv4_tiles(const Kv4Attn& a, int nq, int tile_rows) {
-    const int t = (nq * a.rep + tile_rows - 1) / tile_rows;    // (2^24 rows of 2^6 heads at most: the host's check)
-    return t < a.tiles ? t : a.tiles;                          // max_rows bounds the tiles
+    return (kv4_rows(a, nq) * a.rep + tile_rows - 1) / tile_rows;   // (at most a.tiles; 2^31 rows times heads at most: the host's check)
 }
 DEV int kv4_seq_work(const Kv4Attn& a, int tile_rows, int b) {
     if (b >= a.c.n_seq) return 0;
@@ -562,7 +564,7 @@ template <int G, int NT> __global__ void __launch_bounds__(256, G * NT <= 2 ? 4 
         x = x_end;
         if (in_seq >= tiles * c.n_head_kv) return;
     }
-    const int kvh = uniform_int(in_seq / tiles), tile = in_seq - kvh * tiles, row0 = tile * ROWS, n_rows = nq * a.rep - row0 < ROWS ? nq * a.rep - row0 : ROWS;
+    const int kvh = uniform_int(in_seq / tiles), tile = in_seq - kvh * tiles, row0 = tile * ROWS, all = kv4_rows(a, nq) * a.rep, n_rows = all - row0 < ROWS ? all - row0 : ROWS;
     const bool whole = begin == 0 && end == nb;
 
     u32x4 q[NT][G];
@@ -767,7 +769,7 @@ template <int NR, bool LINE, int W> __global__ void __launch_bounds__(64 * W) kv
     }
     int lo, hi, len;
     kv4_seq(c, b, lo, hi, len);
-    if (row < lo) return;   // (cu does not ascend)
+    if (row < lo || row - lo >= a.max_rows) return;   // (cu does not ascend; rows that are not taken)
     const int kvh = head / a.rep, r = (row - lo) * a.rep + head % a.rep, tile = r / tile_rows, dim = c.head_dim;
     const long long step = (long long)tile_rows * (dim + 2);
     int parts;

@@ -77,6 +77,7 @@ static void rows_vec(Kv4Rows& r) {   // 16-byte loads of dims that lie side by s
 static bool append_grid(Kv4Append& a, int max_rows, dim3& grid, const char*& err) {
     const Kv4Cache& c = a.c;
     if (max_rows > c.total) max_rows = c.total;
+    a.max_rows = max_rows;
     a.blocks = (int)(((long long)max_rows + 62) / 32);
     const long long x = (long long)a.blocks * c.n_seq * c.n_head_kv;
     if (x > 0x7FFFFFFF) { err = "too many rows times sequences for one call"; return false; }
@@ -139,6 +140,7 @@ long long kv4_attention_plan(Kv4Attn& a, int max_rows) {
     const Kv4Cache& c = a.c;
     a.rep = a.n_head / c.n_head_kv;
     if (max_rows > c.total) max_rows = c.total;
+    a.max_rows = max_rows;
     const long long rows = (long long)max_rows * a.rep;
     const int tr = tile_rows(a, rows);
     a.tiles = (int)((rows + tr - 1) / tr);

@@ -25,6 +25,7 @@ struct Kv4Append {
     Kv4Cache c;
     Kv4Rows k, v;
     int blocks;     // most blocks that the new rows of one sequence touch
+    int max_rows;   // rows of a sequence from here on are left out
     int absolute;   // 1: a row's place in k and v is its position in the sequence, not its place among the packed rows (kv4_append_kernel)
 };
 struct Kv4Attn {
@@ -33,7 +34,7 @@ struct Kv4Attn {
     void* out;
     long long o_row, o_head;
     float* ws;               // partial results, head_dim + 2 floats a row: [share][2][rows of a tile] or [row tile][split][rows of a tile]
-    int out_type, n_head, rep, tiles, nsplit, min_blocks, want_parts;   // rep: query heads of a KV head; tiles: row tiles of a (sequence, KV head)
+    int out_type, n_head, rep, tiles, nsplit, min_blocks, want_parts, max_rows;   // rep: query heads of a KV head; tiles: row tiles of a (sequence, KV head); max_rows: as above
     float scale;
 };
 

@@ -190,7 +190,7 @@ def test_results_in_the_queries_place(dev, news):
     c.fill(2)
     pages, table, lens = c.on(dev)
     q = torch.randn((news + 3, 10, 32), generator=torch.Generator().manual_seed(1)).half().to(dev)
-    att = lambda out: ops.kv4_attention(q, pages, table, lens, ints(dev, 0, news, news + 3), news, n_head_kv=2, page_tokens=32, out=out)  # noqa: E731
+    att = lambda out: ops.kv4_attention(q, pages, table, lens, ints(dev, 0, news, news + 3), max(news, 3), n_head_kv=2, page_tokens=32, out=out)  # noqa: E731
     want = att(None)
     assert torch.equal(att(q), want)
 
@@ -264,6 +264,31 @@ def test_a_gradient_is_not_lost_in_silence(dev):
     with torch.no_grad():
         assert torch.equal(att(g), want)
         app(g, x)
+
+
+@pytest.mark.parametrize("news,most", [(7, 3), (40, 1), (40, 33), (300, 130), (200, 50)])
+def test_rows_beyond_max_rows_are_not_processed(dev, news, most):
+    """a sequence with more rows than the call allows: the first of them are those of the whole, the others' places are left as they are"""
+    for width in (1, 10):
+        c = Cache(1, [320 + news, 5], 1, 32, 32, extra_width=width)
+        c.fill(2)
+        cu = ints(dev, 0, news, news + 2)
+        k, v = (torch.randn((news + 2, 1, 32), generator=torch.Generator().manual_seed(i)).half().to(dev) for i in (3, 4))
+        whole, table, lens = c.on(dev)
+        part, old = whole.clone(), whole.clone()
+        ops.kv4_append(k, v, whole, table, lens, cu, news, page_tokens=32)
+        ops.kv4_append(k, v, part, table, lens, cu, most, page_tokens=32)
+        read = lambda p, n: ops.kv4_read(p, table, lens, cu, n, news + 2, n_head_kv=1, head_dim=32, page_tokens=32, dtype=torch.float32)  # noqa: E731
+        new, was = read(whole, news), read(old, news)
+        take = [i < most or i >= news for i in range(news)] + [True, most > 1]
+        here = torch.tensor(take, device=dev)
+        for got, n, w in zip(read(part, news), new, was):
+            assert torch.equal(got[here], n[here]) and torch.equal(got[~here], w[~here])
+        q = torch.randn((news + 2, 3, 32), generator=torch.Generator().manual_seed(5)).half().to(dev)
+        att = lambda n, out: ops.kv4_attention(q, whole, table, lens, cu, n, n_head_kv=1, page_tokens=32, out=out)  # noqa: E731
+        want, got = att(news, None), att(most, torch.full_like(q, 7))
+        assert (got[~here] == 7).all()
+        assert (got[here].float() - want[here].float()).abs().max() < 2.0**-7   # (another kernel may have taken them: values of 1, halves)
 
 
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
