@@ -185,7 +185,7 @@ bool kv4_attention(Kv4Attn& a, int max_rows, long long ws_floats, hipStream_t st
     const Kv4Cache& c = a.c;
     if (a.n_head < 1 || a.n_head > 65536 || a.n_head % c.n_head_kv) { err = "n_head is a multiple of n_head_kv"; return false; }
     if (!(a.scale >= -FLT_MAX && a.scale <= FLT_MAX)) { err = "scale is not a finite number"; return false; }
-    if (a.q.dim != 1) { err = "the dims of a query row are adjacent"; return false; }
+    if (c.total && a.q.dim != 1) { err = "the dims of a query row are adjacent"; return false; }
     if (c.total == 0 || c.n_seq == 0 || max_rows <= 0) return true;
     if (!tables_there(c, err)) return false;
     const long long want = kv4_attention_plan(a, max_rows);
@@ -367,7 +367,7 @@ int ctamd_kv4_attention(const ctamd_kv4_cache* cache, int n_head, const ctamd_ro
     Kv4Attn a = Kv4Attn();
     Kv4Rows o = Kv4Rows();
     bool ok = cache_of(cache, a.c, err) && rows_of(q, a.q, a.c.total, err) && rows_of(out, o, a.c.total, err);
-    if (ok && o.dim != 1) { err = "the dims of an output row are adjacent"; ok = false; }
+    if (ok && a.c.total && o.dim != 1) { err = "the dims of an output row are adjacent"; ok = false; }
     ok = ok && rows_apart(o, a.c.total, n_head, a.c.head_dim, err);
     a.out = (void*)o.p; a.o_row = o.row; a.o_head = o.head; a.out_type = o.type; a.n_head = n_head; a.scale = scale; a.ws = ws;
     ok = ok && ctamd::kv4_attention(a, cache->max_rows, ws_floats, (hipStream_t)stream, err);

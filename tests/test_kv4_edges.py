@@ -291,6 +291,20 @@ def test_rows_beyond_max_rows_are_not_processed(dev, news, most):
         assert (got[here].float() - want[here].float()).abs().max() < 2.0**-7   # (another kernel may have taken them: values of 1, halves)
 
 
+def test_no_rows_of_any_stride(dev):
+    """an empty tensor is contiguous whatever its strides are; there is nothing to do"""
+    c = Cache(1, [40, 3], 2, 64, 32)
+    pages, table, lens = c.on(dev)
+    q = torch.empty((64, 0, 4), dtype=torch.float16, device=dev).permute(1, 2, 0)
+    cu = ints(dev, 0, 0, 0)
+    assert ops.kv4_attention(q, pages, table, lens, cu, 0, n_head_kv=2, page_tokens=32).shape == (0, 4, 64)
+    out = torch.empty((64, 0, 4), dtype=torch.float32, device=dev).permute(1, 2, 0)
+    assert ops.kv4_attention(q, pages, table, lens, cu, 5, n_head_kv=2, page_tokens=32, out=out) is out
+    old = pages.clone()
+    ops.kv4_append(q[:, :2], q[:, 2:], pages, table, lens, cu, 5, page_tokens=32)
+    assert torch.equal(pages, old)
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("length,add", [(2**31 - 1, 2**31 - 1), (1, 2**31 - 1), (2**31 - 1, 1), (2**30, 2**30)])
 def test_room_behind_lengths_near_2_31(dev, length, add):
