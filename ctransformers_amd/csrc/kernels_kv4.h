@@ -227,7 +227,7 @@ DEV const uint8_t* kv4_in_page(const Kv4Cache& c, int pid, int h, int blk) {
 // One workgroup per (block, head) that new rows fall into: it alone writes that block, so a V dword that keeps older tokens is read, changed and written without
 // atomics.  A lane takes eight dims (16 bytes of a half row, so that a wave reads whole lines), four lanes a group; they agree on the largest value by two quad
 // exchanges.  K codes and scales go straight out, V codes cross the workgroup through LDS (eight tokens to a dword).  All loads of a lane are issued before the
-// first value is used.  16 prompts of up to 1500 tokens, 64 heads of 112 in float32 (702 MB in, 113 MB out): 216 us, 3.8 TB/s; one token of 64 sequences, 8 heads:
+// first value is used.  16 prompts of up to 1500 tokens, 64 heads of 112 in float32 (702 MB in, 113 MB out): 217 us, 3.8 TB/s; one token of 64 sequences, 8 heads:
 // 6.4 us, latency (cursor -> table -> rows -> codes -> store).
 template <int G> __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
     __shared__ uint32_t vcode[32][8 * G + 1];   // V codes as bytes [token][dim]; + 1: tokens in different banks
@@ -485,8 +485,8 @@ DEV u32x4 kv4_values(uint32_t w, uint32_t s0, uint32_t s1, uint32_t s2, uint32_t
 // passes it by more than 2^kLag, so most blocks exchange nothing between lanes.  P enters as two halves, the rounded one and what it left (the matrix cores have the time:
 // +2 % at most): off by 2^-22 of p, or 2^-36 of the row's largest where p is smaller than that allows.  V's product with its scale is one half, 2^-11.
 // One sequence of 130 000 tokens, 8 KV heads of 128 with 8 query heads each (150 MB): 35 us, 4.3 TB/s; 64 sequences of 0 .. 8192 tokens (303 MB): 71 us, 4.3 TB/s.  A large
-// copy moves 4.66 TB/s, reading alone reaches 6.4 .. 6.6: memory is not all of it.  Counters of the second: vector units 54 % busy, matrix cores 14 %, 2.1 waves a SIMD,
-// which wait for data 30 % and for their turn to issue 36 % of their time.  One sequence of 140 tokens: 7.3 us, latency.
+// copy moves 4.66 TB/s, reading alone reaches 6.4 .. 6.6: memory is not all of it.  Counters of the second: vector units 56 % busy, matrix cores 14 %, 2.1 waves a SIMD,
+// which wait for data 30 % and for their turn to issue 36 % of their time.  One sequence of 140 tokens: 7.5 us, latency.
 // The next block's K is fetched into the registers of this one's as soon as its scores are there, its V after the V product: 40 dwords a lane at 128 dims for a
 // block in flight, which leaves room for three waves a SIMD (146 registers).
 template <int G> DEV void kv4_fetch_k(uint32_t (&kc)[2][G], uint32_t (&ks)[2][2 * G], const uint8_t* blk, int m, int i) {
@@ -851,7 +851,7 @@ template <int NR, bool LINE, int W> __global__ void __launch_bounds__(64 * W) kv
 // Rounded on the way: K's and V's values and p to halves (2^-11 each at most, p below 2^-25 of the row's largest by up to 2^-36 of that; the 32 x 32 products want halves).  A float16 result is off by 3.8e-4 of its norm, its own
 // rounding alone by 2.1e-4; K exact, as in the kernel above, would take 128 more fused multiply-adds and 32 more LDS reads a step.
 // 2048 tokens, 32 heads of 128 (34 GFLOP): 72 - 81 us, 424 - 477 TFLOP/s; 4 chunks of up to 512 behind up to 8000 tokens, 64 / 8 heads (252 GFLOP): 333 - 391 us, 645 - 758
-// TFLOP/s (a large f16 product: 1142).  Neither pipe is full: counters of the chunks have the vector units 41 % busy and the matrix cores 31 %, with 1.6 waves a SIMD of the two
+// TFLOP/s (a large f16 product: 1142).  Neither pipe is full: counters of the chunks have the vector units 42 % busy and the matrix cores 31 %, with 1.6 waves a SIMD of the two
 // that fit, which wait 33 % of their time (the prompt: 26 %, 18 %, 1.2 waves, 35 %).  What is lost is overlap — 270 vector instructions a step and wave beside 1024 cycles of
 // matrix products — and the ends of launches, where the longest tiles run alone.  Measured and not taken: one block a step and three waves a SIMD (96 / 421 us), unpacking
 // between the K.Q products (82 / 371), wave priorities around them (no change), all pairs' long tiles first (chunks 635).

@@ -4,8 +4,8 @@
 //
 // reserve and compact are two launches each: workgroup 0 of the first plans (a scan over the sequences and the pages: latency, ~1 us per 4096 pages and per 1024 sequences,
 // more where many of those share their last page: each counts those before it among its 1024) while the others copy the tables; the second applies the plan and moves the
-// pages, which is a plain copy and bound by memory.  Moving 424 MB (half of a pool of 16 layers): 190 us, 4.5 TB/s read and written (a large copy: 4.66).  256 sequences of
-// up to 8192 tokens: fork 2.9 + 2.9 us, room for 16 more tokens 11.1 + 4.6 us.
+// pages, which is a plain copy and bound by memory.  Moving 424 MB (half of a pool of 16 layers): 189 us, 4.5 TB/s read and written (a large copy: 4.66).  256 sequences of
+// up to 8192 tokens: fork 3.1 + 2.9 us, room for 16 more tokens 11.3 + 4.6 us.
 #pragma once
 #include "kv4.h"
 
